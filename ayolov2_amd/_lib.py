@@ -13,7 +13,7 @@ _HERE = os.path.dirname(os.path.abspath(__file__))
 # AYOLO_LIB selects another build of the same ABI (A/B timing of two kernel versions on one box: tools/ab_bench.sh)
 LIB_PATH = os.environ.get("AYOLO_LIB") or os.path.join(_HERE, "libayolo_hip.so")
 
-F16, F32 = 0, 1
+F16, F32, BF16 = 0, 1, 2
 EPI_NONE, EPI_AFFINE, EPI_AFFINE_SILU, EPI_HEAD, EPI_AFFINE_RES, EPI_AFFINE_SILU_RES = 0, 1, 2, 3, 4, 5
 
 
@@ -60,6 +60,21 @@ class LossLevel(ctypes.Structure):
                    ("dz", c_void_p), ("ldz", c_int), ("dz_dtype", c_int), ("dbias", c_void_p)])
 
 
+class Rows(ctypes.Structure):
+    """ayolo_rows (include/ayolo.h): where the rows of a layer norm's operand lie."""
+    _fields_ = [("data", c_void_p), ("stride", c_int64), ("outer_stride", c_int64), ("inner", c_int64)]
+
+
+class AdamWList(ctypes.Structure):
+    """ayolo_adamw_list (include/ayolo.h): the tensors of an AdamW step, as arrays that tensor_rows() fills."""
+    _fields_ = [(n, c_char_p) for n in ("p", "g", "m", "v", "me", "ve", "step")] + [("lr", c_char_p), ("weight_decay", c_char_p), ("n", c_int)]
+
+
+class AdamWHyper(ctypes.Structure):
+    _fields_ = ([("beta1", c_double), ("beta2", c_double)] + [(n, c_float) for n in ("eps", "lr", "weight_decay", "max_norm")]
+                + [(n, c_void_p) for n in ("lr_dev", "grad_scale", "found_inf", "norm")] + [("maximize", c_int), ("seed", c_uint32)])
+
+
 class AyoloError(RuntimeError):
     pass
 
@@ -84,6 +99,13 @@ _SIGNATURES = {
     "ayolo_ema_update": [_P, c_int, c_float, _P],
     "ayolo_cast_weights": [_P, c_int, c_int, _P],
     "ayolo_sgd_step": [_P, c_int, _P, _P, _P, _P],
+    "ayolo_grad_norm": [c_char_p, c_int, _P, _P, _P, c_size_t, _P],
+    "ayolo_grad_clip": [c_char_p, c_int, _P, c_float, _P],
+    "ayolo_adamw_step": [POINTER(AdamWList), POINTER(AdamWHyper), _P, c_size_t, _P],
+    "ayolo_moment_values": [c_char_p, c_char_p, c_char_p, c_int, c_int, _P],
+    "ayolo_layer_norm_fwd": [c_int, POINTER(Rows), POINTER(Rows), c_int64, c_int64, _P, _P, c_int, c_float, _P, _P, _P, _P, _P],
+    "ayolo_layer_norm_bwd": [c_int, POINTER(Rows), POINTER(Rows), POINTER(Rows), c_int64, c_int64, _P, c_int, _P, _P, _P, _P, _P, _P,
+                             c_size_t, _P],
     "ayolo_coco_rows": [_P, _P, c_int64, _P, _P, c_int, _P, _P],
     "ayolo_bn_finalize": [_P, c_int, c_int, c_double, _P, _P, c_float, c_float, _P, _P, _P, _P, _P, _P, _P],
     "ayolo_bn_finalize_ld": [_P, c_int, c_int, c_int, c_double, _P, _P, c_float, c_float, _P, _P, _P, _P, _P, _P, _P],
@@ -148,7 +170,15 @@ _SIGNATURES = {
     "ayolo_release_thread_state": [],
 }
 
-EXPORTED = sorted(list(_SIGNATURES) + ["ayolo_version", "ayolo_last_error", "ayolo_conv_wgrad_workspace"])
+# name -> argtypes of the workspace queries (they return a size)
+_SIZES = {
+    "ayolo_conv_wgrad_workspace": [POINTER(ConvDesc)],
+    "ayolo_grad_norm_workspace": [c_char_p, c_int],
+    "ayolo_adamw_workspace": [c_int],
+    "ayolo_layer_norm_bwd_workspace": [c_int, c_int64, c_int64],
+}
+
+EXPORTED = sorted(list(_SIGNATURES) + list(_SIZES) + ["ayolo_version", "ayolo_last_error"])
 
 _lib = None
 
@@ -166,8 +196,10 @@ def lib() -> ctypes.CDLL:
             fn.argtypes = args
             fn.restype = c_int
         l.ayolo_version.restype = c_int
-        l.ayolo_conv_wgrad_workspace.argtypes = [POINTER(ConvDesc)]
-        l.ayolo_conv_wgrad_workspace.restype = c_size_t
+        for name, args in _SIZES.items():
+            fn = getattr(l, name)
+            fn.argtypes = args
+            fn.restype = c_size_t
         l.ayolo_last_error.restype = c_char_p
         _lib = l
     return _lib
@@ -181,6 +213,36 @@ def check(rc: int, what: str) -> None:
 
 def call(name: str, *args) -> None:
     check(getattr(lib(), name)(*args), name)
+
+
+def call_on(device: int, name: str, *args) -> None:
+    """call() with the current stream of device `device` as the last argument, that device being current."""
+    import torch
+    if torch.cuda.current_device() == device:
+        check(getattr(lib(), name)(*args, torch.cuda.current_stream().cuda_stream), name)
+        return
+    with torch.cuda.device(device):
+        check(getattr(lib(), name)(*args, torch.cuda.current_stream().cuda_stream), name)
+
+
+_host = None
+
+
+def tensor_rows(tensors, what: str, item: int = -1) -> bytes:
+    """The ayolo_tensor array of a list of tensors (None: absent), filled by the compiled helper _host.so.  `item` takes that
+    item of every entry (8-bit moments are (codes, exponents) pairs)."""
+    global _host
+    if _host is None:
+        try:
+            from . import _host as mod
+        except ImportError as e:
+            raise AyoloError("ayolov2_amd/_host.so is missing: build it with `python -c 'import __graft_entry__ as g; g.build()'` "
+                             f"(or `make -C ayolov2_amd/csrc`). There is no fallback. ({e})")
+        _host = mod
+    try:
+        return _host.rows(tensors, item)
+    except TypeError as e:
+        raise AyoloError(f"{what}: {e}")
 
 
 def bump_versions(tensors) -> None:

@@ -1,0 +1,693 @@
+// The optimiser's side of a training step over MANY tensors at once, beside the SGD step of optim.hip: the 2-norm of all
+// gradients, their clipping, and AdamW with its two moments in 32 or in 8 bits.
+//
+//   norm = sqrt(sum g^2) / grad_scale            clip: g *= min(1, max_norm / (norm + 1e-6))
+//   t += 1   g' = (+-) g / grad_scale * min(1, max_norm / (norm + 1e-6))
+//   m = b1 m + (1 - b1) g'      v = b2 v + (1 - b2) g'^2
+//   p -= lr wd p + lr / (1 - b1^t) * m / (sqrt(v) / sqrt(1 - b2^t) + eps)
+//
+// Bound: HBM.  Per fp32 parameter 4 B for the norm, 8 B for the clipping, 28 B for AdamW with 32-bit moments and 16 B with 8-bit
+// ones.  The tensors come as a list on the host and travel BY VALUE in the kernel arguments (up to 4 KB per launch: some 80
+// tensors), so nothing is copied to the device, nothing has to be kept between calls, and a captured call replays as it is.
+// A workgroup takes CHUNK elements of one tensor; it finds its tensor with one vector compare and a ballot over the jobs'
+// first workgroups.
+#include "common.h"
+#include <math.h>
+#include <algorithm>
+#include <utility>
+#include <vector>
+
+typedef __bf16 bf16_t;
+typedef unsigned v2u __attribute__((ext_vector_type(2)));
+
+namespace {
+
+constexpr int CHUNK = 4096;                                // elements per workgroup: 256 threads x 4 vectors of 4
+constexpr unsigned PART = 1u << 30;                        // a larger tensor travels as several jobs (a multiple of CHUNK)
+constexpr unsigned MOST_WGS = 1u << 22;                    // of a launch, before its last job (at most 2^18 more): far below 2^32 threads
+
+template <typename T> struct V4 { typedef T type __attribute__((ext_vector_type(4), aligned(sizeof(T)))); };
+template <typename T> __device__ __forceinline__ float4v load4(const T* p) {
+    const typename V4<T>::type r = *reinterpret_cast<const typename V4<T>::type*>(p);
+    return float4v{(float)r[0], (float)r[1], (float)r[2], (float)r[3]};
+}
+template <typename T> __device__ __forceinline__ void store4(T* p, float4v v) {
+    typename V4<T>::type r;
+#pragma unroll
+    for (int e = 0; e < 4; ++e) r[e] = (T)v[e];
+    *reinterpret_cast<typename V4<T>::type*>(p) = r;
+}
+// the first `n` of four elements; the others read as zero and are not written
+template <typename T> __device__ __forceinline__ float4v load_upto(const T* p, int n) {
+    if (n >= 4) return load4(p);
+    float4v v = {0.0f, 0.0f, 0.0f, 0.0f};
+#pragma unroll
+    for (int e = 0; e < 3; ++e)
+        if (e < n) v[e] = (float)p[e];
+    return v;
+}
+template <typename T> __device__ __forceinline__ void store_upto(T* p, float4v v, int n) {
+    if (n >= 4) { store4(p, v); return; }
+#pragma unroll
+    for (int e = 0; e < 3; ++e)
+        if (e < n) p[e] = (T)v[e];
+}
+
+// the job whose workgroups hold this one: `first` ascends, so it is the last job with first <= blockIdx.x
+template <typename JOBS>
+__device__ __forceinline__ int find_job(const JOBS& P) {
+    int j = 0;
+    for (int base = 0; base < P.njobs; base += 64) {
+        const int i = base + (int)(threadIdx.x & 63);
+        const bool below = i < P.njobs && P.j[i < P.njobs ? i : 0].first <= blockIdx.x;
+        j += __popcll(__ballot(below));
+    }
+    return __builtin_amdgcn_readfirstlane(j - 1);
+}
+
+// ------------------------------------------------------------------------------------------------ norm and clipping
+struct GJob { void* g; unsigned n, first; int dtype, pad; };
+struct GJobs {
+    static constexpr int MAX = 160;
+    const float* norm;
+    double* part;
+    float max_norm;
+    int njobs;
+    GJob j[MAX];
+};
+static_assert(sizeof(GJobs) <= 4096, "kernel arguments");
+
+template <typename T>
+__device__ __forceinline__ double squares(const T* g, unsigned n, unsigned at) {
+    double s = 0.0;
+    float4v x[CHUNK / 1024];
+#pragma unroll
+    for (int k = 0; k < CHUNK / 1024; ++k) {
+        const unsigned i = at + k * 1024 + threadIdx.x * 4;
+        x[k] = load_upto(g + (i < n ? i : 0), i < n ? (int)min(n - i, 4u) : 0);
+    }
+#pragma unroll
+    for (int k = 0; k < CHUNK / 1024; ++k)
+#pragma unroll
+        for (int e = 0; e < 4; ++e) s += (double)x[k][e] * (double)x[k][e];
+    return s;
+}
+__device__ __forceinline__ double wave_sum(double v) {
+    for (int d = 1; d < 64; d *= 2) v += __shfl_xor(v, d);
+    return v;
+}
+// one partial sum per workgroup, in fp64: squares of fp32 values neither overflow nor vanish, and the order of the additions
+// does not show in the rounded result.  fp64 runs at half the fp32 rate here and stays far below the memory time.
+__global__ __launch_bounds__(256) void k_grad_squares(GJobs P) {
+    __shared__ double w[4];
+    const int j = find_job(P);
+    const GJob& J = P.j[j];
+    const unsigned at = (blockIdx.x - J.first) * CHUNK;
+    double s = J.dtype == AYOLO_F32   ? squares((const float*)J.g, J.n, at)
+               : J.dtype == AYOLO_F16 ? squares((const half_t*)J.g, J.n, at)
+                                      : squares((const bf16_t*)J.g, J.n, at);
+    s = wave_sum(s);
+    if ((threadIdx.x & 63) == 0) w[threadIdx.x >> 6] = s;
+    __syncthreads();
+    if (threadIdx.x == 0) P.part[blockIdx.x] = (w[0] + w[1]) + (w[2] + w[3]);
+}
+__global__ __launch_bounds__(1024) void k_grad_norm(const double* part, int64_t n, const float* grad_scale, float* out) {
+    __shared__ double w[16];
+    double s = 0.0;
+    for (int64_t i = threadIdx.x; i < n; i += 1024) s += part[i];
+    s = wave_sum(s);
+    if ((threadIdx.x & 63) == 0) w[threadIdx.x >> 6] = s;
+    __syncthreads();
+    if (threadIdx.x == 0) {
+        double t = 0.0;
+        for (int i = 0; i < 16; ++i) t += w[i];
+        t = sqrt(t);
+        *out = (float)(grad_scale ? t / (double)*grad_scale : t);
+    }
+}
+
+// min(1, max_norm / (norm + 1e-6)); a NaN norm gives NaN, as the formula does
+__device__ __forceinline__ float clip_factor(const float* norm, float max_norm) {
+    const float c = max_norm / (*norm + 1e-6f);
+    return c > 1.0f ? 1.0f : c;
+}
+
+template <typename T>
+__device__ __forceinline__ void scale(T* g, unsigned n, unsigned at, float f) {
+    float4v x[CHUNK / 1024];
+#pragma unroll
+    for (int k = 0; k < CHUNK / 1024; ++k) {
+        const unsigned i = at + k * 1024 + threadIdx.x * 4;
+        x[k] = load_upto(g + (i < n ? i : 0), i < n ? (int)min(n - i, 4u) : 0);
+    }
+#pragma unroll
+    for (int k = 0; k < CHUNK / 1024; ++k) {
+        const unsigned i = at + k * 1024 + threadIdx.x * 4;
+        if (i < n) store_upto(g + i, x[k] * f, (int)min(n - i, 4u));
+    }
+}
+__global__ __launch_bounds__(256) void k_grad_clip(GJobs P) {
+    const int j = find_job(P);
+    const GJob& J = P.j[j];
+    const unsigned at = (blockIdx.x - J.first) * CHUNK;
+    const float f = clip_factor(P.norm, P.max_norm);
+    if (J.dtype == AYOLO_F32) scale((float*)J.g, J.n, at, f);
+    else if (J.dtype == AYOLO_F16) scale((half_t*)J.g, J.n, at, f);
+    else scale((bf16_t*)J.g, J.n, at, f);
+}
+
+// -------------------------------------------------------------------------------------------------- 8-bit moments
+// A moment in 8 bits: one byte per element and one exponent byte E per block of 128 elements (memory order), the biased fp32
+// exponent of the block's largest finite magnitude.  m: sign, 4 exponent bits, 3 mantissa bits; v: 5 exponent bits, 3 mantissa
+// bits.  Read as the top bits of an fp32 number (code << 20) and scaled by 2^(E - B), B = 14 (m) or 30 (v): the block's largest
+// value has exponent field B, field B + 1 takes the carry of a rounding up and the codes of infinity and NaN, field 0 holds the
+// subnormals, whose spacing fp32's own subnormals give without a branch.
+//
+// The ranges fit each other: m keeps 2^-17 of its block's largest value, v 2^-33 (sqrt: 2^-16.5), and a v above zero never
+// becomes zero, so that the smallest kept m over the smallest kept sqrt(v) stays a step of ordinary size.
+//
+// Rounding is stochastic, E[stored] = value: at b2 = 0.999 a step moves v by 0.1 % and a 3-bit mantissa by 6 % or nothing, so
+// that rounding to nearest would hold v where it first was.  16 random bits (and a half of the next) per rounding come from a
+// hash of (seed, t, position of the tensor, element): a call's result depends on its arguments alone.
+constexpr int M_BIAS = 14, V_BIAS = 30, M_LEAST = 1, V_LEAST = 10;      // least E: keeps every value a multiple of 2^-149
+
+__device__ __forceinline__ unsigned mix(unsigned x) {
+    x ^= x >> 16;
+    x *= 0x6A09E667u;                                      // odd: the first bits of the fractions of sqrt(2) and sqrt(3)
+    x ^= x >> 15;
+    x *= 0xBB67AE85u;
+    return x ^ (x >> 16);
+}
+constexpr unsigned STRIDE = 0x9E3779B1u;                   // 2^32 / golden ratio, odd
+
+template <bool SIGNED>
+__device__ __forceinline__ float decode(unsigned code, int e) {
+    const unsigned mag = SIGNED ? code & 0x7fu : code, top = SIGNED ? 0x7fu : 0xffu;
+    float x = __builtin_ldexpf(__uint_as_float(mag << 20), e - (SIGNED ? M_BIAS : V_BIAS));
+    if (mag >= top - 1) x = mag == top ? __uint_as_float(0x7fc00000u) : __uint_as_float(0x7f800000u);
+    return SIGNED && (code & 0x80u) ? -x : x;
+}
+template <bool SIGNED>
+__device__ __forceinline__ unsigned encode(float x, int e, unsigned r16) {
+    const unsigned top = SIGNED ? 0x7fu : 0xffu, bits = __float_as_uint(x) & 0x7fffffffu;
+    const float y = __builtin_ldexpf(__uint_as_float(bits), (SIGNED ? M_BIAS : V_BIAS) - e);
+    unsigned code = (__float_as_uint(y) + (r16 << 4 | 8u)) >> 20;
+    if (!SIGNED && code == 0 && bits != 0) code = 1;
+    if (bits >= 0x7f800000u) code = bits == 0x7f800000u ? top - 1 : top;
+    return SIGNED && x < 0.0f ? code | 0x80u : code;
+}
+// the largest over the 32 lanes of a block, in all of them
+template <int CTRL> __device__ __forceinline__ int dpp_max(int v) {
+    return max(v, __builtin_amdgcn_update_dpp(0, v, CTRL, 0xf, 0xf, true));
+}
+__device__ __forceinline__ int block_max(int v) {
+    v = dpp_max<0xB1>(v);
+    v = dpp_max<0x4E>(v);
+    v = dpp_max<0x141>(v);
+    v = dpp_max<0x140>(v);
+    const v2u r = __builtin_amdgcn_permlane16_swap((unsigned)v, (unsigned)v, false, false);
+    return max((int)r[0], (int)r[1]);
+}
+__device__ __forceinline__ int block_exponent(float4v x, int least) {
+    int e = least;
+#pragma unroll
+    for (int k = 0; k < 4; ++k) {
+        const int f = (int)(__float_as_uint(x[k]) >> 23 & 255u);
+        e = f < 255 && f > e ? f : e;
+    }
+    return block_max(e);
+}
+__device__ __forceinline__ unsigned load_codes(const uint8_t* p, int n) {
+    typedef unsigned u1 __attribute__((aligned(1)));
+    if (n >= 4) return *reinterpret_cast<const u1*>(p);
+    unsigned c = 0;
+#pragma unroll
+    for (int e = 0; e < 3; ++e)
+        if (e < n) c |= (unsigned)p[e] << 8 * e;
+    return c;
+}
+__device__ __forceinline__ void store_codes(uint8_t* p, unsigned c, int n) {
+    typedef unsigned u1 __attribute__((aligned(1)));
+    if (n >= 4) { *reinterpret_cast<u1*>(p) = c; return; }
+#pragma unroll
+    for (int e = 0; e < 3; ++e)
+        if (e < n) p[e] = (uint8_t)(c >> 8 * e);
+}
+template <bool SIGNED>
+__device__ __forceinline__ float4v decode4(unsigned c, int e) {
+    return float4v{decode<SIGNED>(c & 255u, e), decode<SIGNED>(c >> 8 & 255u, e), decode<SIGNED>(c >> 16 & 255u, e), decode<SIGNED>(c >> 24, e)};
+}
+
+// ----------------------------------------------------------------------------------------------------------- AdamW
+struct Coef { float step, decay, root; unsigned key; };    // lr / (1 - b1^t), lr wd, 1 / sqrt(1 - b2^t), the tensor's random key
+
+struct PrepJobs {
+    static constexpr int MAX = 240;
+    double ln_b1, ln_b2;
+    const float *lr, *found_inf;
+    Coef* out;
+    unsigned seed;
+    int n, base, pad;
+    struct { float* step; float lr, wd; } j[MAX];
+};
+static_assert(sizeof(PrepJobs) <= 4096, "kernel arguments");
+
+// One thread per tensor: count the step and leave what depends on it to the update kernels.  1 - b^t in fp64: for b = 0.999 and
+// the first steps an fp32 difference would keep few of its bits.
+__global__ __launch_bounds__(256) void k_adamw_prepare(PrepJobs P) {
+    const int i = threadIdx.x;
+    if (i >= P.n || !P.j[i].step) return;
+    if (P.found_inf && *P.found_inf != 0.0f) return;
+    const float t = *P.j[i].step + 1.0f;
+    *P.j[i].step = t;
+    const double lr = P.lr ? (double)*P.lr : (double)P.j[i].lr;
+    Coef c;
+    c.step = (float)(lr / -expm1((double)t * P.ln_b1));
+    c.decay = (float)(lr * (double)P.j[i].wd);
+    c.root = (float)(1.0 / sqrt(-expm1((double)t * P.ln_b2)));
+    c.key = mix(mix(P.seed + STRIDE * (unsigned)t) + STRIDE * (unsigned)(P.base + i + 1));
+    P.out[P.base + i] = c;
+}
+
+struct Hyper {
+    const float *grad_scale, *found_inf, *norm;
+    const Coef* coef;
+    float b1, c1, b2, c2, eps, max_norm;
+    int maximize;
+};
+template <bool BITS8> struct AJob;
+template <> struct AJob<false> { void* p; const void* g; float *m, *v; unsigned n, first, tensor, origin; };
+template <> struct AJob<true> { void* p; const void* g; uint8_t *m, *v, *me, *ve; unsigned n, first, tensor, origin; };
+template <bool BITS8> struct AJobs {
+    static constexpr int MAX = BITS8 ? 60 : 80;
+    Hyper h;
+    int njobs, pad;
+    AJob<BITS8> j[MAX];
+};
+static_assert(sizeof(AJobs<false>) <= 4096 && sizeof(AJobs<true>) <= 4096, "kernel arguments");
+
+struct Scalars { float scale, factor, sign; bool scaled; };
+__device__ __forceinline__ float4v true_grad(float4v g, const Scalars& c) {
+    if (c.scaled)
+#pragma unroll
+        for (int e = 0; e < 4; ++e) g[e] = g[e] / c.scale;
+    return g * (c.sign * c.factor);
+}
+// the moments, one rounding per operation (compiled without contraction): a plain sequence of the formula's products and sums
+__device__ __forceinline__ void moments(float4v g, const Hyper& h, float4v& m, float4v& v) {
+    m = m * h.b1 + g * h.c1;
+    v = v * h.b2 + g * g * h.c2;
+}
+__device__ __forceinline__ float4v stepped(float4v p, float4v m, float4v v, const Coef& c, float eps) {
+#pragma unroll
+    for (int e = 0; e < 4; ++e) {
+        const float d = __builtin_fmaf(sqrtf(v[e]), c.root, eps);
+        p[e] -= __builtin_fmaf(p[e], c.decay, c.step * (m[e] / d));
+    }
+    return p;
+}
+
+template <typename T, bool BITS8>
+__global__ __launch_bounds__(256) void k_adamw(AJobs<BITS8> P) {
+    const Hyper& h = P.h;
+    if (h.found_inf && *h.found_inf != 0.0f) return;
+    const int j = find_job(P);
+    const AJob<BITS8>& J = P.j[j];
+    const Coef c = h.coef[J.tensor];
+    Scalars sc;
+    sc.scaled = h.grad_scale != nullptr;
+    sc.scale = sc.scaled ? *h.grad_scale : 1.0f;
+    sc.factor = h.norm ? clip_factor(h.norm, h.max_norm) : 1.0f;
+    sc.sign = h.maximize ? -1.0f : 1.0f;
+    const unsigned at = (blockIdx.x - J.first) * CHUNK;
+    T* p = (T*)J.p;
+    const T* g = (const T*)J.g;
+    constexpr int U = CHUNK / 1024;
+    float4v x[U], d[U];
+    int left[U];
+    unsigned pos[U];
+#pragma unroll
+    for (int k = 0; k < U; ++k) {
+        const unsigned i = at + k * 1024 + threadIdx.x * 4;
+        left[k] = i < J.n ? (int)min(J.n - i, 4u) : 0;
+        pos[k] = i < J.n ? i : 0;
+        x[k] = load_upto(p + pos[k], left[k]);
+        d[k] = load_upto(g + pos[k], left[k]);
+    }
+    if constexpr (!BITS8) {
+        float4v m[U], v[U];
+#pragma unroll
+        for (int k = 0; k < U; ++k) {
+            m[k] = load_upto(J.m + pos[k], left[k]);
+            v[k] = load_upto(J.v + pos[k], left[k]);
+        }
+#pragma unroll
+        for (int k = 0; k < U; ++k) {
+            moments(true_grad(d[k], sc), h, m[k], v[k]);
+            if (left[k] > 0) {
+                store_upto(p + pos[k], stepped(x[k], m[k], v[k], c, h.eps), left[k]);
+                store_upto(J.m + pos[k], m[k], left[k]);
+                store_upto(J.v + pos[k], v[k], left[k]);
+            }
+        }
+    } else {
+        unsigned mc[U], vc[U];
+        int me[U], ve[U];
+#pragma unroll
+        for (int k = 0; k < U; ++k) {                      // 32 lanes hold one block of 128
+            mc[k] = load_codes(J.m + pos[k], left[k]);
+            vc[k] = load_codes(J.v + pos[k], left[k]);
+            me[k] = J.me[pos[k] / 128];
+            ve[k] = J.ve[pos[k] / 128];
+        }
+#pragma unroll
+        for (int k = 0; k < U; ++k) {
+            float4v m = decode4<true>(mc[k], me[k]), v = decode4<false>(vc[k], ve[k]);
+            moments(true_grad(d[k], sc), h, m, v);
+#pragma unroll
+            for (int e = 0; e < 4; ++e)                    // past the end: not part of the block
+                if (e >= left[k]) m[e] = v[e] = 0.0f;
+            const int em = block_exponent(m, M_LEAST), ev = block_exponent(v, V_LEAST);
+            if (left[k] > 0) store_upto(p + pos[k], stepped(x[k], m, v, c, h.eps), left[k]);
+            unsigned cm = 0, cv = 0;
+#pragma unroll
+            for (int e = 0; e < 4; ++e) {
+                const unsigned r = mix(((J.origin + pos[k] + e) * STRIDE) ^ c.key);
+                cm |= encode<true>(m[e], em, r >> 16) << 8 * e;
+                cv |= encode<false>(v[e], ev, r & 0xffffu) << 8 * e;
+            }
+            if (left[k] > 0) {
+                store_codes(J.m + pos[k], cm, left[k]);
+                store_codes(J.v + pos[k], cv, left[k]);
+                if ((threadIdx.x & 31) == 0) {
+                    J.me[pos[k] / 128] = (uint8_t)em;
+                    J.ve[pos[k] / 128] = (uint8_t)ev;
+                }
+            }
+        }
+    }
+}
+
+struct UJob { const uint8_t *codes, *exps; float* out; unsigned n, first; };
+struct UJobs {
+    static constexpr int MAX = 120;
+    int njobs, pad;
+    UJob j[MAX];
+};
+static_assert(sizeof(UJobs) <= 4096, "kernel arguments");
+template <bool SIGNED>
+__global__ __launch_bounds__(256) void k_moment_values(UJobs P) {
+    const int j = find_job(P);
+    const UJob& J = P.j[j];
+    const unsigned at = (blockIdx.x - J.first) * CHUNK;
+    constexpr int U = CHUNK / 1024;
+    unsigned c[U];
+    int e[U];
+#pragma unroll
+    for (int k = 0; k < U; ++k) {
+        const unsigned i = at + k * 1024 + threadIdx.x * 4, pos = i < J.n ? i : 0;
+        c[k] = load_codes(J.codes + pos, i < J.n ? (int)min(J.n - i, 4u) : 0);
+        e[k] = J.exps[pos / 128];
+    }
+#pragma unroll
+    for (int k = 0; k < U; ++k) {
+        const unsigned i = at + k * 1024 + threadIdx.x * 4;
+        if (i < J.n) store_upto(J.out + i, decode4<SIGNED>(c[k], e[k]), (int)min(J.n - i, 4u));
+    }
+}
+
+// ------------------------------------------------------------------------------------------------------------- host
+int es_of(int dtype) { return dtype == AYOLO_F32 ? 4 : dtype == AYOLO_U8 ? 1 : 2; }
+bool is_float(int dtype) { return dtype == AYOLO_F32 || dtype == AYOLO_F16 || dtype == AYOLO_BF16; }
+
+// every tensor of the list is a dense block of device memory of one device, of a type that `ok` takes
+template <typename OK>
+int check_list(const char* what, const char* name, const ayolo_tensor* t, int n, int& device, OK ok) {
+    for (int i = 0; i < n; ++i) {
+        if (!t[i].present) continue;
+        AY_CHECK_ARG(t[i].device >= 0, "%s: %s[%d] is not on a GPU (the HIP path has no CPU fallback)", what, name, i);
+        if (device < 0) device = t[i].device;
+        AY_CHECK_ARG(t[i].device == device, "%s: %s[%d] is on device %d, others on %d", what, name, i, t[i].device, device);
+        AY_CHECK_ARG(ok(t[i].dtype), "%s: %s[%d] has an unsupported type", what, name, i);
+        AY_CHECK_ARG(t[i].layout != 0, "%s: %s[%d] is not a dense block of memory", what, name, i);
+        AY_CHECK_ARG(t[i].numel == 0 || t[i].data, "%s: %s[%d] has no memory", what, name, i);
+        AY_CHECK_ARG((uintptr_t)t[i].data % es_of(t[i].dtype) == 0, "%s: %s[%d] is not aligned to its type", what, name, i);
+    }
+    return AYOLO_OK;
+}
+struct Ranges {
+    std::vector<std::pair<uintptr_t, uintptr_t>> r;
+    void add(const ayolo_tensor* t, int n) {
+        for (int i = 0; i < n; ++i)
+            if (t[i].present && t[i].numel > 0) r.emplace_back((uintptr_t)t[i].data, (uintptr_t)t[i].data + (uintptr_t)t[i].numel * es_of(t[i].dtype));
+    }
+    bool overlap() {
+        std::sort(r.begin(), r.end());
+        for (size_t i = 1; i < r.size(); ++i)
+            if (r[i].first < r[i - 1].second) return true;
+        return false;
+    }
+};
+
+// Splits a list into launches: `put(job, offset, count)` fills one job, `go(jobs, workgroups)` launches what has gathered.
+template <typename JOBS, typename PUT, typename GO>
+int each_launch(JOBS& P, const ayolo_tensor* t, int n, PUT put, GO go) {
+    unsigned wgs = 0;
+    P.njobs = 0;
+    auto flush = [&]() -> int {
+        if (P.njobs == 0) return AYOLO_OK;
+        const int rc = go(P, wgs);
+        P.njobs = 0;
+        wgs = 0;
+        return rc;
+    };
+    for (int i = 0; i < n; ++i) {
+        if (!t[i].present) continue;
+        for (int64_t off = 0; off < t[i].numel; off += PART) {
+            const unsigned cnt = (unsigned)std::min<int64_t>(PART, t[i].numel - off);
+            if (P.njobs == JOBS::MAX || wgs >= MOST_WGS) {
+                if (const int rc = flush()) return rc;
+            }
+            auto& J = P.j[P.njobs];
+            if (const int rc = put(J, i, off, flush)) return rc;
+            auto& K = P.j[P.njobs];                        // `put` may have flushed
+            K = J;
+            K.n = cnt;
+            K.first = wgs;
+            wgs += (cnt + CHUNK - 1) / CHUNK;
+            ++P.njobs;
+        }
+    }
+    return flush();
+}
+
+int64_t chunks_of(const ayolo_tensor* t, int n) {
+    int64_t c = 0;
+    for (int i = 0; i < n; ++i)
+        if (t[i].present)
+            for (int64_t off = 0; off < t[i].numel; off += PART) c += cdiv64(std::min<int64_t>(PART, t[i].numel - off), CHUNK);
+    return c;
+}
+
+}  // namespace
+
+extern "C" size_t ayolo_grad_norm_workspace(const ayolo_tensor* grads, int n) {
+    return grads && n > 0 ? (size_t)std::max<int64_t>(chunks_of(grads, n), 1) * sizeof(double) : sizeof(double);
+}
+
+extern "C" int ayolo_grad_norm(const ayolo_tensor* grads, int n, const float* grad_scale, float* norm, void* ws, size_t ws_bytes, ayolo_stream st) {
+    AY_CHECK_ARG(n >= 0 && (n == 0 || grads) && norm, "grad_norm: null argument");
+    int dev = -1;
+    if (const int rc = check_list("grad_norm", "grads", grads, n, dev, is_float)) return rc;
+    const int64_t chunks = chunks_of(grads, n);
+    if (!ws || ws_bytes < ayolo_grad_norm_workspace(grads, n)) { ayolo_set_error("grad_norm: workspace %zu < %zu", ws_bytes, ayolo_grad_norm_workspace(grads, n)); return AYOLO_ENOSPC; }
+    hipStream_t s = (hipStream_t)st;
+    GJobs P{};
+    P.part = (double*)ws;
+    const int rc = each_launch(P, grads, n,
+        [&](GJob& J, int i, int64_t off, auto&&) { J.g = (char*)grads[i].data + off * es_of(grads[i].dtype); J.dtype = grads[i].dtype; return AYOLO_OK; },
+        [&](GJobs& Q, unsigned wgs) {
+            hipLaunchKernelGGL(k_grad_squares, dim3(wgs), dim3(256), 0, s, Q);
+            Q.part += wgs;
+            AY_CHECK_LAUNCH("k_grad_squares");
+            return AYOLO_OK;
+        });
+    if (rc) return rc;
+    hipLaunchKernelGGL(k_grad_norm, dim3(1), dim3(1024), 0, s, (const double*)ws, chunks, grad_scale, norm);
+    AY_CHECK_LAUNCH("k_grad_norm");
+    return AYOLO_OK;
+}
+
+extern "C" int ayolo_grad_clip(const ayolo_tensor* grads, int n, const float* norm, float max_norm, ayolo_stream st) {
+    AY_CHECK_ARG(n >= 0 && (n == 0 || grads) && norm && max_norm >= 0.0f, "grad_clip: null argument or max_norm=%g", (double)max_norm);
+    int dev = -1;
+    if (const int rc = check_list("grad_clip", "grads", grads, n, dev, is_float)) return rc;
+    try {
+        Ranges r;
+        r.add(grads, n);
+        AY_CHECK_ARG(!r.overlap(), "grad_clip: two of the gradients share memory");
+    } catch (...) { ayolo_set_error("grad_clip: out of host memory"); return AYOLO_ENOSPC; }
+    hipStream_t s = (hipStream_t)st;
+    GJobs P{};
+    P.norm = norm;
+    P.max_norm = max_norm;
+    return each_launch(P, grads, n,
+        [&](GJob& J, int i, int64_t off, auto&&) { J.g = (char*)grads[i].data + off * es_of(grads[i].dtype); J.dtype = grads[i].dtype; return AYOLO_OK; },
+        [&](GJobs& Q, unsigned wgs) {
+            hipLaunchKernelGGL(k_grad_clip, dim3(wgs), dim3(256), 0, s, Q);
+            AY_CHECK_LAUNCH("k_grad_clip");
+            return AYOLO_OK;
+        });
+}
+
+namespace {
+template <bool BITS8>
+int adamw_launches(const ayolo_adamw_list& L, const Hyper& h, hipStream_t s) {
+    AJobs<BITS8> P{};
+    P.h = h;
+    int dtype = -1;                                        // of the jobs that have gathered
+    auto go = [&](AJobs<BITS8>& Q, unsigned wgs) {
+        if (dtype == AYOLO_F32) hipLaunchKernelGGL((k_adamw<float, BITS8>), dim3(wgs), dim3(256), 0, s, Q);
+        else if (dtype == AYOLO_F16) hipLaunchKernelGGL((k_adamw<half_t, BITS8>), dim3(wgs), dim3(256), 0, s, Q);
+        else hipLaunchKernelGGL((k_adamw<bf16_t, BITS8>), dim3(wgs), dim3(256), 0, s, Q);
+        AY_CHECK_LAUNCH("k_adamw");
+        return AYOLO_OK;
+    };
+    auto put = [&](AJob<BITS8>& J, int i, int64_t off, auto&& flush) {
+        if (L.p[i].dtype != dtype) {
+            if (const int rc = flush()) return rc;
+            dtype = L.p[i].dtype;
+        }
+        const int es = es_of(dtype);
+        J.p = (char*)L.p[i].data + off * es;
+        J.g = (const char*)L.g[i].data + off * es;
+        if constexpr (BITS8) {
+            J.m = (uint8_t*)L.m[i].data + off;
+            J.v = (uint8_t*)L.v[i].data + off;
+            J.me = (uint8_t*)L.me[i].data + off / 128;
+            J.ve = (uint8_t*)L.ve[i].data + off / 128;
+        } else {
+            J.m = (float*)L.m[i].data + off;
+            J.v = (float*)L.v[i].data + off;
+        }
+        J.tensor = (unsigned)i;
+        J.origin = (unsigned)off;
+        return AYOLO_OK;
+    };
+    return each_launch(P, L.g, L.n, put, go);
+}
+}  // namespace
+
+extern "C" size_t ayolo_adamw_workspace(int n) { return n > 0 ? (size_t)n * sizeof(Coef) : sizeof(Coef); }
+
+extern "C" int ayolo_adamw_step(const ayolo_adamw_list* L, const ayolo_adamw_hyper* H, void* ws, size_t ws_bytes, ayolo_stream st) {
+    AY_CHECK_ARG(L && H && L->n >= 0, "adamw_step: null argument");
+    const int n = L->n;
+    if (n == 0) return AYOLO_OK;
+    AY_CHECK_ARG(L->p && L->g && L->m && L->v && L->step && !L->me == !L->ve, "adamw_step: null list");
+    const bool bits8 = L->me != nullptr;
+    AY_CHECK_ARG(H->beta1 >= 0.0 && H->beta1 < 1.0 && H->beta2 >= 0.0 && H->beta2 < 1.0, "adamw_step: betas=(%g, %g)", H->beta1, H->beta2);
+    AY_CHECK_ARG(H->eps >= 0.0f, "adamw_step: eps=%g", (double)H->eps);
+    AY_CHECK_ARG(!H->norm || H->max_norm >= 0.0f, "adamw_step: max_norm=%g", (double)H->max_norm);
+    int dev = -1;
+    auto is_f32 = [](int d) { return d == AYOLO_F32; };
+    auto is_state = [&](int d) { return d == (bits8 ? AYOLO_U8 : AYOLO_F32); };
+    auto is_u8 = [](int d) { return d == AYOLO_U8; };
+    if (const int rc = check_list("adamw_step", "params", L->p, n, dev, is_float)) return rc;
+    if (const int rc = check_list("adamw_step", "grads", L->g, n, dev, is_float)) return rc;
+    if (const int rc = check_list("adamw_step", "exp_avgs", L->m, n, dev, is_state)) return rc;
+    if (const int rc = check_list("adamw_step", "exp_avg_sqs", L->v, n, dev, is_state)) return rc;
+    if (const int rc = check_list("adamw_step", "steps", L->step, n, dev, is_f32)) return rc;
+    if (bits8) {
+        if (const int rc = check_list("adamw_step", "exponents of exp_avgs", L->me, n, dev, is_u8)) return rc;
+        if (const int rc = check_list("adamw_step", "exponents of exp_avg_sqs", L->ve, n, dev, is_u8)) return rc;
+    }
+    for (int i = 0; i < n; ++i) {
+        if (!L->g[i].present) continue;
+        const ayolo_tensor &p = L->p[i], &g = L->g[i], &m = L->m[i], &v = L->v[i];
+        AY_CHECK_ARG(p.present && m.present && v.present && L->step[i].present, "adamw_step: tensor %d has a gradient and no parameter, state or step", i);
+        AY_CHECK_ARG(g.dtype == p.dtype, "adamw_step: tensor %d: the gradient's type is not the parameter's", i);
+        AY_CHECK_ARG(g.numel == p.numel && m.numel == p.numel && v.numel == p.numel, "adamw_step: tensor %d: sizes differ", i);
+        AY_CHECK_ARG(g.layout == p.layout && m.layout == p.layout && v.layout == p.layout, "adamw_step: tensor %d: gradient or state in another shape or memory order than the parameter", i);
+        AY_CHECK_ARG(L->step[i].numel == 1, "adamw_step: steps[%d] is not one number", i);
+        if (bits8) {
+            const int64_t nb = cdiv64(p.numel, 128);
+            AY_CHECK_ARG(L->me[i].present && L->ve[i].present && L->me[i].numel == nb && L->ve[i].numel == nb, "adamw_step: tensor %d needs %lld exponents", i, (long long)nb);
+        }
+    }
+    try {
+        Ranges r;
+        r.add(L->p, n);
+        r.add(L->m, n);
+        r.add(L->v, n);
+        r.add(L->step, n);
+        if (bits8) { r.add(L->me, n); r.add(L->ve, n); }
+        AY_CHECK_ARG(!r.overlap(), "adamw_step: two of the parameters, states or steps share memory");
+    } catch (...) { ayolo_set_error("adamw_step: out of host memory"); return AYOLO_ENOSPC; }
+    const size_t need = ayolo_adamw_workspace(n);
+    if (!ws || ws_bytes < need) { ayolo_set_error("adamw_step: workspace %zu < %zu", ws_bytes, need); return AYOLO_ENOSPC; }
+    hipStream_t s = (hipStream_t)st;
+    PrepJobs Q{};
+    Q.ln_b1 = log(H->beta1);
+    Q.ln_b2 = log(H->beta2);
+    Q.lr = H->lr_dev;
+    Q.found_inf = H->found_inf;
+    Q.out = (Coef*)ws;
+    Q.seed = H->seed;
+    for (int base = 0; base < n; base += PrepJobs::MAX) {
+        Q.base = base;
+        Q.n = std::min(n - base, (int)PrepJobs::MAX);
+        bool any = false;
+        for (int i = 0; i < Q.n; ++i) {
+            const bool on = L->g[base + i].present;
+            any |= on;
+            Q.j[i].step = on ? (float*)L->step[base + i].data : nullptr;
+            Q.j[i].lr = L->lr ? L->lr[base + i] : H->lr;
+            Q.j[i].wd = L->weight_decay ? L->weight_decay[base + i] : H->weight_decay;
+        }
+        if (!any) continue;
+        hipLaunchKernelGGL(k_adamw_prepare, dim3(1), dim3(256), 0, s, Q);
+        AY_CHECK_LAUNCH("k_adamw_prepare");
+    }
+    Hyper h{};
+    h.grad_scale = H->grad_scale;
+    h.found_inf = H->found_inf;
+    h.norm = H->norm;
+    h.coef = (const Coef*)ws;
+    h.b1 = (float)H->beta1;
+    h.c1 = (float)(1.0 - H->beta1);
+    h.b2 = (float)H->beta2;
+    h.c2 = (float)(1.0 - H->beta2);
+    h.eps = H->eps;
+    h.max_norm = H->max_norm;
+    h.maximize = H->maximize;
+    return bits8 ? adamw_launches<true>(*L, h, s) : adamw_launches<false>(*L, h, s);
+}
+
+extern "C" int ayolo_moment_values(const ayolo_tensor* codes, const ayolo_tensor* exps, const ayolo_tensor* out, int n, int is_signed, ayolo_stream st) {
+    AY_CHECK_ARG(n >= 0 && (n == 0 || (codes && exps && out)), "moment_values: null list");
+    int dev = -1;
+    auto is_u8 = [](int d) { return d == AYOLO_U8; };
+    if (const int rc = check_list("moment_values", "codes", codes, n, dev, is_u8)) return rc;
+    if (const int rc = check_list("moment_values", "exponents", exps, n, dev, is_u8)) return rc;
+    if (const int rc = check_list("moment_values", "out", out, n, dev, [](int d) { return d == AYOLO_F32; })) return rc;
+    for (int i = 0; i < n; ++i) {
+        AY_CHECK_ARG(codes[i].present && exps[i].present && out[i].present, "moment_values: tensor %d is missing", i);
+        AY_CHECK_ARG(out[i].numel == codes[i].numel && out[i].layout == codes[i].layout && exps[i].numel == cdiv64(codes[i].numel, 128), "moment_values: tensor %d: sizes or memory orders differ", i);
+    }
+    hipStream_t s = (hipStream_t)st;
+    UJobs P{};
+    return each_launch(P, codes, n,
+        [&](UJob& J, int i, int64_t off, auto&&) {
+            J.codes = (const uint8_t*)codes[i].data + off;
+            J.exps = (const uint8_t*)exps[i].data + off / 128;
+            J.out = (float*)out[i].data + off;
+            return AYOLO_OK;
+        },
+        [&](UJobs& Q, unsigned wgs) {
+            if (is_signed) hipLaunchKernelGGL(k_moment_values<true>, dim3(wgs), dim3(256), 0, s, Q);
+            else hipLaunchKernelGGL(k_moment_values<false>, dim3(wgs), dim3(256), 0, s, Q);
+            AY_CHECK_LAUNCH("k_moment_values");
+            return AYOLO_OK;
+        });
+}

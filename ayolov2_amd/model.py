@@ -20,7 +20,7 @@ import torch
 import yaml
 from torch import nn
 
-from .modules import C3, SPPF, Bottleneck, Concat, Conv, UpSample, YOLOHead
+from .modules import C3, SPPF, Bottleneck, Concat, Conv, LayerNorm, UpSample, YOLOHead
 
 
 def make_divisible(x: float, divisor: int = 8) -> int:
@@ -81,6 +81,9 @@ class YOLOModel(nn.Module):
                 out = make_divisible(args[0] * width)
                 m = SPPF(cin[0], out, args[1] if len(args) > 1 else 5, activation=act)
                 cout, r = out, rin[0]
+            elif name == "LayerNorm":                # over the channels; a model that has one runs module by module
+                m = LayerNorm(cin[0], args[0] if len(args) > 0 else 1e-5)
+                cout, r = cin[0], rin[0]
             elif name == "UpSample":
                 m = UpSample(args[0] if len(args) > 0 else None, args[1] if len(args) > 1 else 2)
                 cout, r = cin[0], rin[0] // 2 if rin[0] > 1 else rin[0]

@@ -204,6 +204,24 @@ class SPPF(nn.Module):
         return self.cv2(torch.cat((x, y1, y2, self.pool(y2)), dim=1))
 
 
+class LayerNorm(nn.Module):
+    """Layer norm with a gain and an optional bias: over the channels of every pixel of an activation (dim=1, the yaml's
+    ``LayerNorm`` row), or over the last dimension of tokens (dim=-1).  ``forward(x, residual)`` returns the norm of x + residual
+    and that sum."""
+
+    def __init__(self, channels: int, eps: float = 1e-5, bias: bool = True, dim: int = 1) -> None:
+        super().__init__()
+        self.eps, self.dim = float(eps), int(dim)
+        self.weight = nn.Parameter(torch.ones(channels))
+        self.bias = nn.Parameter(torch.zeros(channels)) if bias else None
+
+    def forward(self, x: torch.Tensor, residual: Optional[torch.Tensor] = None):
+        return F_.layer_norm(x, self.weight, self.bias, self.eps, residual, self.dim)
+
+    def extra_repr(self) -> str:
+        return f"{self.weight.shape[0]}, eps={self.eps}, dim={self.dim}, bias={self.bias is not None}"
+
+
 class UpSample(nn.Module):
     def __init__(self, size=None, scale_factor=2, mode: str = "nearest") -> None:
         super().__init__()

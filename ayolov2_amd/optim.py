@@ -6,11 +6,17 @@ The reference builds ``optim.SGD(pg_bn, lr, momentum, nesterov=True)`` plus a we
 entries, LR schedulers, ``GradScaler.step`` (``_step_supports_amp_scaling``: the scaler hands over ``grad_scale`` and
 ``found_inf`` tensors and the kernel divides / skips on the device, no host sync) -- but the ~180 parameter tensors are
 updated by a single kernel instead of several torch launches per parameter group.  CPU parameters fall back to
-torch's own arithmetic (the class is then a plain torch.optim.SGD)."""
+torch's own arithmetic (the class is then a plain torch.optim.SGD).
+
+``AdamW``, ``adamw_step``: torch.optim.AdamW's step over many tensors at once (``ayolo_adamw_step``), moments in 32 or in 8 bits;
+``grad_norm``, ``clip_grads_``, ``clip_grad_norm_``: the 2-norm of all gradients and clipping by it (``ayolo_grad_norm``,
+``ayolo_grad_clip``).  These take their tensors as lists and keep nothing between calls, so a captured call replays as it is."""
 from __future__ import annotations
 
+import array
 import ctypes
-from typing import Optional
+import math
+from typing import NamedTuple, Optional, Sequence, Tuple, Union
 
 import numpy as np
 import torch
@@ -146,3 +152,311 @@ class SGD(torch.optim.SGD):
                   torch.cuda.current_stream().cuda_stream)
         _lib.bump_versions(p for (_, p), g in zip(plist, grads) if g is not None)     # written through raw pointers
         return loss
+
+
+# ---------------------------------------------------------------------------------------- gradient norm and clipping
+_TENSOR = np.dtype([("data", "<u8"), ("numel", "<i8"), ("layout", "<u8"), ("dtype", "<i4"), ("device", "<i2"), ("present", "<i2")])
+MOMENT_BLOCK = 128          # elements of an 8-bit moment that share an exponent
+
+
+def _device_of(tensors, what: str) -> torch.device:
+    for t in tensors:
+        if t is not None:
+            if not t.is_cuda:
+                raise _lib.AyoloError(f"{what}: the HIP path needs tensors on the GPU (got {t.device}); there is no CPU fallback")
+            return t.device
+    return None
+
+
+def _scalar(t: Optional[torch.Tensor], dev: torch.device, what: str, name: str):
+    """The address of one fp32 number on the device (None: a null pointer)."""
+    if t is None:
+        return None
+    if not torch.is_tensor(t) or t.dtype != torch.float32 or t.numel() != 1 or t.device != dev:
+        raise _lib.AyoloError(f"{what}: {name} must be one fp32 number on {dev}")
+    return t.data_ptr()
+
+
+def grad_norm(grads: Sequence[Optional[torch.Tensor]], grad_scale: Optional[torch.Tensor] = None) -> torch.Tensor:
+    """The 2-norm over all elements of all gradients (fp32, fp16 or bf16; None entries are skipped) as one fp32 number on their
+    device, divided by the device scalar `grad_scale` if given.  Summed in fp64 in a fixed order."""
+    grads = list(grads)
+    dev = _device_of(grads, "grad_norm")
+    if dev is None:
+        return torch.zeros(())
+    rows = _lib.tensor_rows(grads, "grad_norm")
+    info = np.frombuffer(rows, dtype=_TENSOR)
+    if ((info["layout"] == 0) & (info["present"] != 0)).any():       # an expanded or strided gradient: its elements in a block
+        grads = [g if g is None else g.contiguous() for g in grads]
+        rows = _lib.tensor_rows(grads, "grad_norm")
+    need = int(_lib.lib().ayolo_grad_norm_workspace(rows, len(grads)))
+    ws = torch.empty(need, dtype=torch.uint8, device=dev)
+    norm = torch.empty((), dtype=torch.float32, device=dev)
+    _lib.call_on(dev.index, "ayolo_grad_norm", rows, len(grads), _scalar(grad_scale, dev, "grad_norm", "grad_scale"), norm.data_ptr(),
+                 ws.data_ptr(), need)
+    return norm
+
+
+def clip_grads_(grads: Sequence[Optional[torch.Tensor]], max_norm: float, norm: Optional[torch.Tensor] = None) -> torch.Tensor:
+    """Multiplies every gradient by ``min(1, max_norm / (norm + 1e-6))`` in place and returns the norm (a device scalar; computed
+    here unless given).  An infinite norm makes finite gradients zero, a NaN norm makes all of them NaN, as the formula does.
+    Gradients must be dense blocks of memory that do not overlap."""
+    grads = list(grads)
+    max_norm = float(max_norm)
+    if not max_norm >= 0.0:
+        raise _lib.AyoloError(f"clip_grads_: max_norm={max_norm}")
+    dev = _device_of(grads, "clip_grads_")
+    if dev is None:
+        return torch.zeros(()) if norm is None else norm
+    if norm is None:
+        norm = grad_norm(grads)
+    _lib.call_on(dev.index, "ayolo_grad_clip", _lib.tensor_rows(grads, "clip_grads_"), len(grads), _scalar(norm, dev, "clip_grads_", "norm"),
+                 max_norm)
+    _lib.bump_versions(grads)
+    return norm
+
+
+def clip_grad_norm_(parameters, max_norm: float, norm_type: float = 2.0, error_if_nonfinite: bool = False) -> torch.Tensor:
+    """torch.nn.utils.clip_grad_norm_ for the 2-norm: clips the parameters' ``.grad`` in place (three launches per hundred and
+    sixty tensors) and returns their norm.  Gradients on the CPU go to torch's own function."""
+    if float(norm_type) != 2.0:
+        raise _lib.AyoloError(f"clip_grad_norm_: norm_type={norm_type}: only the 2-norm has a kernel")
+    parameters = [parameters] if torch.is_tensor(parameters) else list(parameters)
+    grads = [p.grad for p in parameters if p.grad is not None]
+    if not grads or not grads[0].is_cuda:
+        return torch.nn.utils.clip_grad_norm_(parameters, max_norm, norm_type, error_if_nonfinite)
+    norm = grad_norm(grads)
+    if error_if_nonfinite and not bool(torch.isfinite(norm)):
+        raise RuntimeError("clip_grad_norm_: the gradients' norm is not finite")
+    with torch.no_grad():
+        return clip_grads_(grads, max_norm, norm)
+
+
+# --------------------------------------------------------------------------------------------------------------- AdamW
+class Moment8(NamedTuple):
+    """A moment in 8 bits: one code per element in the parameter's shape and memory order, one exponent per MOMENT_BLOCK codes."""
+    codes: torch.Tensor
+    exps: torch.Tensor
+
+
+def new_moment8(p: torch.Tensor) -> Moment8:
+    """An 8-bit moment of zeros for parameter `p`."""
+    return Moment8(torch.zeros_like(p, dtype=torch.uint8, memory_format=torch.preserve_format),
+                   torch.zeros(-(-p.numel() // MOMENT_BLOCK), dtype=torch.uint8, device=p.device))
+
+
+def unpack_moments(moments: Sequence[Moment8], signed: bool, out: Optional[Sequence[torch.Tensor]] = None) -> Sequence[torch.Tensor]:
+    """The fp32 values of 8-bit moments, all in one go.  `signed`: first moments (exp_avg), else second ones (exp_avg_sq)."""
+    moments = list(moments)
+    if not moments:
+        return [] if out is None else out
+    dev = _device_of((m[0] for m in moments), "unpack_moments")
+    if out is None:
+        out = [torch.empty_like(m[0], dtype=torch.float32) for m in moments]
+    elif len(out) != len(moments):
+        raise _lib.AyoloError(f"unpack_moments: {len(out)} outputs for {len(moments)} moments")
+    _lib.call_on(dev.index, "ayolo_moment_values", _lib.tensor_rows(moments, "unpack_moments", 0), _lib.tensor_rows(moments, "unpack_moments", 1),
+                 _lib.tensor_rows(out, "unpack_moments"), len(moments), int(bool(signed)))
+    _lib.bump_versions(out)
+    return out
+
+
+def _per_tensor(v, n: int, what: str):
+    """(number, None), or (0, n floats as bytes) where a number per tensor is given."""
+    if isinstance(v, (int, float)):
+        if not (math.isfinite(v) and v >= 0.0):
+            raise _lib.AyoloError(f"adamw_step: {what}={v}")
+        return float(v), None
+    arr = array.array("f", v)
+    if len(arr) != n:
+        raise _lib.AyoloError(f"adamw_step: {len(arr)} values of {what} for {n} tensors")
+    if not all(0.0 <= x < math.inf for x in arr):
+        raise _lib.AyoloError(f"adamw_step: {what} must be finite and not negative")
+    return 0.0, arr.tobytes()
+
+
+def adamw_step(params: Sequence[torch.Tensor], grads: Sequence[Optional[torch.Tensor]], exp_avgs: Sequence, exp_avg_sqs: Sequence,
+               steps: Sequence[torch.Tensor], *, lr: Union[float, torch.Tensor, Sequence[float]], betas: Tuple[float, float] = (0.9, 0.999),
+               eps: float = 1e-8, weight_decay: Union[float, Sequence[float]] = 1e-2, maximize: bool = False, seed: int = 0,
+               total_norm: Optional[torch.Tensor] = None, max_norm: Optional[float] = None, grad_scale: Optional[torch.Tensor] = None,
+               found_inf: Optional[torch.Tensor] = None) -> None:
+    """One AdamW step (torch.optim.AdamW's arithmetic) over lists of tensors, in place, in a few launches for all of them.
+
+    params / grads: fp32, fp16 or bf16 on one GPU, a gradient of its parameter's type (None: that entry stays as it is); dense
+    blocks of memory, states in the parameter's memory order.  16-bit parameters are rounded to nearest: what is below half a
+    step of theirs is lost, so keep fp32 masters for long training.  exp_avgs / exp_avg_sqs: fp32 tensors, or Moment8 pairs
+    (new_moment8), rounded stochastically from `seed`, the step, the entry's place in the list and the element.  steps: one fp32
+    number per entry on the device, counted up here.  lr: a number, a number per tensor, or a device scalar (which a captured
+    step follows); weight_decay: a number, or a number per tensor.  total_norm with max_norm: gradients are multiplied by
+    min(1, max_norm / (total_norm + 1e-6)) on the way.  grad_scale: a device scalar that gradients are divided by; found_inf: a
+    device scalar, nothing at all is changed where it is not 0 (torch.amp.GradScaler's pair)."""
+    params, grads = list(params), list(grads)
+    n = len(params)
+    for other, name in ((grads, "grads"), (exp_avgs, "exp_avgs"), (exp_avg_sqs, "exp_avg_sqs"), (steps, "steps")):
+        if len(other) != n:
+            raise _lib.AyoloError(f"adamw_step: {len(other)} {name} for {n} params")
+    dev = _device_of(grads, "adamw_step")
+    if dev is None:
+        return
+    if (total_norm is None) != (max_norm is None):
+        raise _lib.AyoloError("adamw_step: total_norm and max_norm go together")
+    kinds = {isinstance(m, (tuple, list)) for l in (exp_avgs, exp_avg_sqs) for m, g in zip(l, grads) if g is not None}
+    if len(kinds) != 1:
+        raise _lib.AyoloError("adamw_step: moments of 8 and of 32 bits in one call")
+    bits8 = kinds.pop()
+    rows = _lib.tensor_rows
+    L, H = _lib.AdamWList(), _lib.AdamWHyper()
+    prows, grows = rows(params, "adamw_step: params"), rows(grads, "adamw_step: grads")
+    pi, gi = np.frombuffer(prows, dtype=_TENSOR), np.frombuffer(grows, dtype=_TENSOR)
+    other = (gi["present"] != 0) & (pi["layout"] != gi["layout"])
+    if other.any():                                # a gradient in another memory order than its parameter: laid out like it
+        for i in np.flatnonzero(other):
+            if torch.is_tensor(params[i]) and params[i].shape == grads[i].shape:
+                grads[i] = SGD._dense_like(params[i], grads[i])
+        grows = rows(grads, "adamw_step: grads")
+    L.n, L.p, L.g = n, prows, grows
+    if bits8:
+        L.m, L.me = rows(exp_avgs, "adamw_step: exp_avgs", 0), rows(exp_avgs, "adamw_step: exp_avgs", 1)
+        L.v, L.ve = rows(exp_avg_sqs, "adamw_step: exp_avg_sqs", 0), rows(exp_avg_sqs, "adamw_step: exp_avg_sqs", 1)
+    else:
+        L.m, L.v = rows(exp_avgs, "adamw_step: exp_avgs"), rows(exp_avg_sqs, "adamw_step: exp_avg_sqs")
+    L.step = rows(steps, "adamw_step: steps")
+    if torch.is_tensor(lr):
+        H.lr_dev = _scalar(lr, dev, "adamw_step", "lr")
+    else:
+        H.lr, L.lr = _per_tensor(lr, n, "lr")
+    H.weight_decay, L.weight_decay = _per_tensor(weight_decay, n, "weight_decay")
+    H.beta1, H.beta2, H.eps = float(betas[0]), float(betas[1]), float(eps)
+    H.grad_scale = _scalar(grad_scale, dev, "adamw_step", "grad_scale")
+    H.found_inf = _scalar(found_inf, dev, "adamw_step", "found_inf")
+    H.norm = _scalar(total_norm, dev, "adamw_step", "total_norm")
+    H.max_norm = 0.0 if max_norm is None else float(max_norm)
+    H.maximize, H.seed = int(bool(maximize)), int(seed) & 0xFFFFFFFF
+    need = int(_lib.lib().ayolo_adamw_workspace(n))
+    ws = torch.empty(need, dtype=torch.uint8, device=dev)
+    _lib.call_on(dev.index, "ayolo_adamw_step", L, H, ws.data_ptr(), need)
+    _lib.bump_versions(p for p, g in zip(params, grads) if g is not None)         # written through raw pointers
+
+
+class AdamW(torch.optim.AdamW):
+    """torch.optim.AdamW's interface and arithmetic with the whole step in a few launches (adamw_step).
+
+    ``state_bits=8`` keeps both moments in one byte per element (``exp_avg`` / ``exp_avg_sq`` hold codes, ``exp_avg_exps`` /
+    ``exp_avg_sq_exps`` an exponent per 128): 2 bytes of state per parameter instead of 8, rounded stochastically from `seed`.
+    ``max_norm`` clips the gradients' global 2-norm inside the step, without writing them.  ``step`` counts on the device, so
+    GradScaler's skipped steps do not count and need no host sync, and a step can be captured (after one eager step, which makes
+    the states; a learning rate that changes between replays is given as a device scalar).  32-bit state dicts and
+    torch.optim.AdamW's load into each other; an 8-bit state dict also loads into a 32-bit optimiser.  CPU parameters fall back
+    to torch's own arithmetic (32-bit states)."""
+    _step_supports_amp_scaling = True
+
+    def __init__(self, params, lr=1e-3, betas=(0.9, 0.999), eps=1e-8, weight_decay=1e-2, *, maximize=False, state_bits=32,
+                 max_norm: Optional[float] = None, seed: int = 0):
+        if state_bits not in (8, 32):
+            raise _lib.AyoloError(f"ayolov2_amd.optim.AdamW: state_bits={state_bits}: 8 or 32")
+        if max_norm is not None and not float(max_norm) >= 0.0:
+            raise _lib.AyoloError(f"ayolov2_amd.optim.AdamW: max_norm={max_norm}")
+        self.state_bits, self.max_norm, self.seed = state_bits, max_norm, seed
+        super().__init__(params, lr=lr, betas=betas, eps=eps, weight_decay=weight_decay, maximize=maximize)
+
+    def __getstate__(self):
+        return {**super().__getstate__(), "state_bits": self.state_bits, "max_norm": self.max_norm, "seed": self.seed}
+
+    def _new_states(self, todo) -> None:
+        """States of parameters that have a gradient for the first time."""
+        if torch.cuda.is_current_stream_capturing():
+            raise _lib.AyoloError("ayolov2_amd.optim.AdamW: run one step before capturing: a replay would start from new states")
+        for (p, st), t in zip(todo, torch.zeros(len(todo), dtype=torch.float32, device=todo[0][0].device).unbind()):
+            st["step"] = t
+            if self.state_bits == 8:
+                m, v = new_moment8(p), new_moment8(p)
+                st["exp_avg"], st["exp_avg_exps"], st["exp_avg_sq"], st["exp_avg_sq_exps"] = m.codes, m.exps, v.codes, v.exps
+            else:
+                st["exp_avg"] = torch.zeros_like(p, dtype=torch.float32, memory_format=torch.preserve_format)
+                st["exp_avg_sq"] = torch.zeros_like(p, dtype=torch.float32, memory_format=torch.preserve_format)
+
+    def _moments(self, st):
+        if not st:
+            return None, None, None
+        if self.state_bits == 8:
+            return Moment8(st["exp_avg"], st["exp_avg_exps"]), Moment8(st["exp_avg_sq"], st["exp_avg_sq_exps"]), st["step"]
+        return st["exp_avg"], st["exp_avg_sq"], st["step"]
+
+    @torch.no_grad()
+    def step(self, closure=None):
+        scale, found = getattr(self, "grad_scale", None), getattr(self, "found_inf", None)
+        on_gpu = {p.is_cuda for g in self.param_groups for p in g["params"] if p.grad is not None}
+        if len(on_gpu) == 2:
+            raise _lib.AyoloError("ayolov2_amd.optim.AdamW: parameters on the CPU and on the GPU")
+        if on_gpu == {False}:
+            if self.state_bits == 8 or scale is not None or found is not None:
+                raise _lib.AyoloError("ayolov2_amd.optim.AdamW: 8-bit states and the GradScaler hand-over need parameters on the GPU")
+            if self.max_norm is not None:
+                if closure is not None:
+                    raise _lib.AyoloError("ayolov2_amd.optim.AdamW: max_norm with a closure needs parameters on the GPU")
+                torch.nn.utils.clip_grad_norm_([p for g in self.param_groups for p in g["params"]], self.max_norm)
+            return super().step(closure)
+        loss = None
+        if closure is not None:
+            with torch.enable_grad():
+                loss = closure()
+        runs, todo, grads = {}, [], []
+        for k, g in enumerate(self.param_groups):
+            if g.get("amsgrad"):
+                raise _lib.AyoloError("ayolov2_amd.optim.AdamW: amsgrad has no kernel")
+            lr = g["lr"]
+            if torch.is_tensor(lr) and not lr.is_cuda:
+                lr = float(lr)
+            # groups that differ in learning rate and decay alone share their launches
+            key = (tuple(g["betas"]), g["eps"], bool(g["maximize"]), k if torch.is_tensor(lr) else -1)
+            run = runs.setdefault(key, ([], [], [], [], lr))
+            for p in g["params"]:
+                st = self.state[p] if p.grad is not None else self.state.get(p, {})
+                if p.grad is not None:
+                    if p.grad.is_sparse:
+                        raise _lib.AyoloError("ayolov2_amd.optim.AdamW: sparse gradients have no kernel")
+                    if not st:
+                        todo.append((p, st))
+                    grads.append(p.grad)
+                run[0].append(p)
+                run[1].append(st)
+                run[2].append(lr)
+                run[3].append(g["weight_decay"])
+        if not grads:
+            return loss
+        if todo:
+            self._new_states(todo)
+        norm = grad_norm(grads, scale) if self.max_norm is not None else None
+        for r, (key, (ps, sts, lrs, wds, lr)) in enumerate(runs.items()):
+            ms, vs, ts = zip(*(self._moments(st) for st in sts)) if ps else ((), (), ())
+            # the seeds of several runs differ, so that their roundings do not repeat one another's
+            adamw_step(ps, [p.grad for p in ps], ms, vs, ts, lr=lr if torch.is_tensor(lr) else lrs, betas=key[0], eps=key[1],
+                       weight_decay=wds, maximize=key[2], seed=self.seed + 0x51F15EED * r, total_norm=norm,
+                       max_norm=self.max_norm if norm is not None else None, grad_scale=scale, found_inf=found)
+        return loss
+
+    def load_state_dict(self, state_dict):
+        super().load_state_dict(state_dict)
+        # the base class has cast every state to its parameter's type: take them again as they were saved
+        ids = [i for g in state_dict["param_groups"] for i in g["params"]]
+        for i, p in zip(ids, (p for g in self.param_groups for p in g["params"])):
+            raw = state_dict["state"].get(i)
+            if not raw or not p.is_cuda:
+                continue
+            st = self.state[p]
+            st["step"] = torch.as_tensor(raw["step"], dtype=torch.float32).detach().reshape(()).to(p.device, copy=True)
+            if self.state_bits == 8 and "exp_avg_exps" not in raw:
+                raise _lib.AyoloError("ayolov2_amd.optim.AdamW: a state dict with 32-bit moments does not load into 8-bit states")
+            for name, signed in (("exp_avg", True), ("exp_avg_sq", False)):
+                if "exp_avg_exps" in raw:
+                    codes = torch.empty_like(p, dtype=torch.uint8, memory_format=torch.preserve_format)
+                    codes.copy_(raw[name])
+                    m = Moment8(codes, raw[name + "_exps"].to(p.device, copy=True))
+                    if self.state_bits == 8:
+                        st[name], st[name + "_exps"] = m
+                    else:
+                        st[name] = unpack_moments([m], signed)[0]
+                        st.pop(name + "_exps", None)
+                else:
+                    st[name] = torch.empty_like(p, dtype=torch.float32, memory_format=torch.preserve_format)
+                    st[name].copy_(raw[name])

@@ -327,8 +327,9 @@ class TrainModelBuilder:
             dist.init_process_group(backend=backend)
 
     def to_ddp(self) -> nn.Module:
+        from .modules import LayerNorm
         if self.cuda and type(self.model).__name__ == "YOLOModel" and getattr(self.model, "use_plan", True) \
-                and os.getenv("AYOLO_TORCH_DDP") != "1":
+                and not any(isinstance(m, LayerNorm) for m in self.model.modules()) and os.getenv("AYOLO_TORCH_DDP") != "1":
             return FlatGradDDP(self.model, sync_bn=bool(self.cfg.get("train", {}).get("sync_bn", False)))
         if self.cuda and self.cfg.get("train", {}).get("sync_bn", False):
             raise NotImplementedError("sync_bn needs the plan executor (YOLOModel with use_plan): the per-module HIP path keeps "
@@ -348,9 +349,11 @@ class TrainModelBuilder:
 
 
 def training_step(model: nn.Module, loss_fn, optimizer: torch.optim.Optimizer, scaler, imgs: torch.Tensor,
-                  targets: torch.Tensor, world_size: int = 1, amp: bool = True, ema: Optional["ModelEMA"] = None):
+                  targets: torch.Tensor, world_size: int = 1, amp: bool = True, ema: Optional["ModelEMA"] = None,
+                  max_norm: Optional[float] = None):
     """autocast forward -> ComputeLoss -> (x world_size under DDP) -> scaled backward -> step (accumulate = 1) -> EMA
-    (yolo_trainer.py:322-338)."""
+    (yolo_trainer.py:322-338).  `max_norm` clips the gradients' global 2-norm before the step (optim.clip_grad_norm_; the
+    reference does not clip).  An optim.AdamW that has a max_norm of its own clips inside its step instead."""
     from ._lib import roctx_range
     with roctx_range("train.forward+loss"), torch.autocast(imgs.device.type, dtype=torch.float16, enabled=amp and imgs.is_cuda):
         pred = model(imgs)
@@ -363,6 +366,11 @@ def training_step(model: nn.Module, loss_fn, optimizer: torch.optim.Optimizer, s
         else:
             loss.backward()
     with roctx_range("train.optimizer"):
+        if max_norm is not None:
+            from .optim import clip_grad_norm_
+            if scaler is not None:
+                scaler.unscale_(optimizer)
+            clip_grad_norm_([p for g in optimizer.param_groups for p in g["params"]], max_norm)
         if scaler is not None:
             scaler.step(optimizer)
             scaler.update()

@@ -34,6 +34,8 @@ extern "C" {
 
 #define AYOLO_F16 0
 #define AYOLO_F32 1
+#define AYOLO_BF16 2        /* layer norm and the optimiser's tensors only */
+#define AYOLO_U8 3          /* 8-bit moments only                          */
 
 typedef void* ayolo_stream; /* hipStream_t */
 
@@ -217,6 +219,72 @@ typedef struct ayolo_sgd_group { float lr, momentum, weight_decay, dampening; in
 typedef struct ayolo_sgd_groups { ayolo_sgd_group g[AYOLO_SGD_MAX_GROUPS]; } ayolo_sgd_groups;
 int ayolo_sgd_step(const ayolo_sgd_job* jobs_dev, int njobs, const ayolo_sgd_groups* groups, const float* grad_scale,
                    const float* found_inf, ayolo_stream s);
+
+/* A tensor of a list that lies on the HOST: the functions below read the list before they return and pass its entries to the
+ * kernels by value.  layout: 0 = not one dense block of memory, else equal for equal shapes in equal memory order. */
+typedef struct ayolo_tensor {
+    void* data;
+    int64_t numel;
+    uint64_t layout;
+    int32_t dtype;        /* AYOLO_F32 | _F16 | _BF16 | _U8, -1: another                            */
+    int16_t device;       /* device ordinal, -1: host memory                                        */
+    int16_t present;      /* 0: the list has no tensor here (a parameter without gradient)          */
+} ayolo_tensor;
+
+/* Gradient clipping by the 2-norm over all tensors (torch.nn.utils.clip_grad_norm_), beside the optimiser step of
+ * scripts/train/yolo_trainer.py:332-338.  ayolo_grad_norm: *norm = sqrt(sum of all squares) / *grad_scale (nullable), summed in
+ * fp64 in a fixed order (no atomics), through a workspace of the size that the query gives.  ayolo_grad_clip: every gradient
+ * *= min(1, max_norm / (*norm + 1e-6)) in place; refused where two tensors of the list overlap.  n = 0 is allowed. */
+size_t ayolo_grad_norm_workspace(const ayolo_tensor* grads, int n);
+int ayolo_grad_norm(const ayolo_tensor* grads, int n, const float* grad_scale, float* norm, void* ws, size_t ws_bytes,
+                    ayolo_stream s);
+int ayolo_grad_clip(const ayolo_tensor* grads, int n, const float* norm, float max_norm, ayolo_stream s);
+
+/* Multi-tensor AdamW step (torch.optim.AdamW's arithmetic, decoupled weight decay) with torch.amp.GradScaler's contract as in
+ * ayolo_sgd_step.  Parameter and gradient: fp32, fp16 or bf16 (both the same; 16-bit parameters are rounded to nearest).
+ * Moments m, v: fp32, or 8-bit codes (me / ve not NULL) with one exponent byte per 128 elements in memory order, rounded
+ * stochastically from `seed`, the step count, the tensor's place in the list and the element.  step: one fp32 number per
+ * tensor on the device, counted up by the call unless *found_inf != 0.  norm (nullable): gradients are multiplied by
+ * min(1, max_norm / (*norm + 1e-6)) on the way, *norm being the norm AFTER division by *grad_scale.  lr_dev (nullable): the
+ * learning rate is read from the device (a captured step follows it).  ws: ayolo_adamw_workspace(n) bytes. */
+typedef struct ayolo_adamw_list {
+    const ayolo_tensor *p, *g, *m, *v, *me, *ve, *step;
+    const float *lr, *weight_decay;       /* host, one per tensor; NULL: the values in ayolo_adamw_hyper */
+    int n;
+} ayolo_adamw_list;
+typedef struct ayolo_adamw_hyper {
+    double beta1, beta2;
+    float eps, lr, weight_decay, max_norm;
+    const float *lr_dev, *grad_scale, *found_inf, *norm;     /* device, each nullable */
+    int maximize;
+    unsigned seed;
+} ayolo_adamw_hyper;
+size_t ayolo_adamw_workspace(int n);
+int ayolo_adamw_step(const ayolo_adamw_list* list, const ayolo_adamw_hyper* hyper, void* ws, size_t ws_bytes, ayolo_stream s);
+/* The fp32 values that 8-bit moments stand for (is_signed: a first moment, else a second one). */
+int ayolo_moment_values(const ayolo_tensor* codes, const ayolo_tensor* exps, const ayolo_tensor* out, int n, int is_signed,
+                        ayolo_stream s);
+
+/* Layer norm over the last dimension of `rows` rows of C elements (tokens, or the channels of an NHWC activation's pixels):
+ * y = (s - mean(s)) * rstd * weight + bias with s = x, or s = x + residual rounded to the activations' type and written to
+ * `sum`.  y and sum are dense [rows][C]; x and residual are addressed through ayolo_rows: elements 1 apart in a row, any row
+ * stride, any alignment.  weight / bias: C elements of fp32 or of the activations' type, nullable.  mean / rstd: float[rows]
+ * for backward, both or neither.  dtype: AYOLO_F16 | _F32 | _BF16; every sum is fp32.
+ * Backward: dx (nullable) = gradient of s plus dsum (the gradient that reaches `sum` itself, nullable); dweight / dbias
+ * (nullable, of wdtype) are sums over the rows in a fixed order, through a workspace of the size that the query gives (used
+ * where one of them is wanted). */
+typedef struct ayolo_rows {
+    const void* data;
+    int64_t stride;        /* elements from a row to the next                                        */
+    int64_t outer_stride;  /* elements from a group of `inner` rows to the next                      */
+    int64_t inner;         /* 0: one group                                                           */
+} ayolo_rows;
+int ayolo_layer_norm_fwd(int dtype, const ayolo_rows* x, const ayolo_rows* residual, int64_t rows, int64_t C, const void* weight,
+                         const void* bias, int wdtype, float eps, void* y, void* sum, float* mean, float* rstd, ayolo_stream s);
+size_t ayolo_layer_norm_bwd_workspace(int dtype, int64_t rows, int64_t C);
+int ayolo_layer_norm_bwd(int dtype, const ayolo_rows* sum, const ayolo_rows* dy, const ayolo_rows* dsum, int64_t rows, int64_t C,
+                         const void* weight, int wdtype, const float* mean, const float* rstd, void* dx, void* dweight,
+                         void* dbias, void* ws, size_t ws_bytes, ayolo_stream s);
 
 /* The same cast for every layer of a model in one launch.  `jobs_dev` is a DEVICE array (written once by the caller;
  * each entry must have Cout_pad*taps*Cin_pad < 2^32). */
