@@ -228,19 +228,27 @@ def call_on(device: int, name: str, *args) -> None:
 _host = None
 
 
-def tensor_rows(tensors, what: str, item: int = -1) -> bytes:
-    """The ayolo_tensor array of a list of tensors (None: absent), filled by the compiled helper _host.so.  `item` takes that
-    item of every entry (8-bit moments are (codes, exponents) pairs)."""
+def host():
+    """The compiled helper _host.so (csrc/host.cpp), bound to this library."""
     global _host
     if _host is None:
+        l = lib()
         try:
             from . import _host as mod
         except ImportError as e:
             raise AyoloError("ayolov2_amd/_host.so is missing: build it with `python -c 'import __graft_entry__ as g; g.build()'` "
                              f"(or `make -C ayolov2_amd/csrc`). There is no fallback. ({e})")
+        mod.bind(AyoloError, *(ctypes.cast(f, c_void_p).value for f in (l.ayolo_layer_norm_fwd, l.ayolo_layer_norm_bwd,
+                                                                       l.ayolo_layer_norm_bwd_workspace, l.ayolo_last_error)))
         _host = mod
+    return _host
+
+
+def tensor_rows(tensors, what: str, item: int = -1) -> bytes:
+    """The ayolo_tensor array of a list of tensors (None: absent).  `item` takes that item of every entry (8-bit moments are
+    (codes, exponents) pairs)."""
     try:
-        return _host.rows(tensors, item)
+        return host().rows(tensors, item)
     except TypeError as e:
         raise AyoloError(f"{what}: {e}")
 

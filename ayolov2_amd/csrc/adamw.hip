@@ -435,14 +435,24 @@ int check_list(const char* what, const char* name, const ayolo_tensor* t, int n,
     }
     return AYOLO_OK;
 }
+// Whether two of the tensors share memory.  Each list is checked as it comes in: lists made in one go ascend, and then the lists
+// need only be merged; otherwise all are sorted.
 struct Ranges {
-    std::vector<std::pair<uintptr_t, uintptr_t>> r;
+    typedef std::pair<uintptr_t, uintptr_t> R;
+    std::vector<R> r;
+    std::vector<size_t> ends;
     void add(const ayolo_tensor* t, int n) {
         for (int i = 0; i < n; ++i)
             if (t[i].present && t[i].numel > 0) r.emplace_back((uintptr_t)t[i].data, (uintptr_t)t[i].data + (uintptr_t)t[i].numel * es_of(t[i].dtype));
+        ends.push_back(r.size());
     }
     bool overlap() {
-        std::sort(r.begin(), r.end());
+        size_t from = 0;
+        for (size_t to : ends) {
+            if (!std::is_sorted(r.begin() + from, r.begin() + to)) std::sort(r.begin() + from, r.begin() + to);
+            if (from > 0 && to > from && r[from] < r[from - 1]) std::inplace_merge(r.begin(), r.begin() + from, r.begin() + to);
+            from = to;
+        }
         for (size_t i = 1; i < r.size(); ++i)
             if (r[i].first < r[i - 1].second) return true;
         return false;
@@ -602,7 +612,12 @@ extern "C" int ayolo_adamw_step(const ayolo_adamw_list* L, const ayolo_adamw_hyp
         if (const int rc = check_list("adamw_step", "exponents of exp_avgs", L->me, n, dev, is_u8)) return rc;
         if (const int rc = check_list("adamw_step", "exponents of exp_avg_sqs", L->ve, n, dev, is_u8)) return rc;
     }
+    auto number = [](float x) { return x >= 0.0f && x < INFINITY; };
+    AY_CHECK_ARG(H->lr_dev || L->lr || number(H->lr), "adamw_step: lr=%g", (double)H->lr);
+    AY_CHECK_ARG(L->weight_decay || number(H->weight_decay), "adamw_step: weight_decay=%g", (double)H->weight_decay);
     for (int i = 0; i < n; ++i) {
+        AY_CHECK_ARG(H->lr_dev || !L->lr || number(L->lr[i]), "adamw_step: lr[%d]=%g", i, (double)L->lr[i]);
+        AY_CHECK_ARG(!L->weight_decay || number(L->weight_decay[i]), "adamw_step: weight_decay[%d]=%g", i, (double)L->weight_decay[i]);
         if (!L->g[i].present) continue;
         const ayolo_tensor &p = L->p[i], &g = L->g[i], &m = L->m[i], &v = L->v[i];
         AY_CHECK_ARG(p.present && m.present && v.present && L->step[i].present, "adamw_step: tensor %d has a gradient and no parameter, state or step", i);

@@ -1,14 +1,42 @@
-// CPython helper of the tensor-list operators (gradient norm, clipping, AdamW): one pass over a Python list of tensors that
-// fills the ayolo_tensor array the C ABI takes.  A model has some hundred tensors in five lists per step; asking each for its
-// address, size, type and strides from Python costs more host time than the step costs the GPU.  No arithmetic here.
+// CPython helper of the operators whose host side is hot: one pass over a Python list of tensors that fills the ayolo_tensor
+// array the C ABI takes (gradient norm, clipping, AdamW: a model has some hundred tensors in five lists per step), and layer
+// norm's checks, buffers and autograd node (a norm of a few rows takes the GPU 3 us, a node written in Python 25 us of host time
+// forward and, in autograd's own thread, 40 us backward).  No arithmetic here: the kernels are reached through the C ABI, whose
+// addresses bind() is given.
+#include <torch/csrc/autograd/custom_function.h>
+#include <torch/csrc/autograd/functions/basic_ops.h>
+#include <torch/csrc/Exceptions.h>
 #include <torch/csrc/autograd/python_variable.h>
+
+#include <ATen/ATen.h>
+#include <c10/core/DeviceGuard.h>
+#include <c10/hip/HIPStream.h>
+
+#include <stdexcept>
+#include <string>
 
 #include "../../include/ayolo.h"
 
 namespace {
 
+using at::Tensor;
+using torch::autograd::AutogradContext;
+using torch::autograd::variable_list;
+
+PyObject* ayolo_error = nullptr;      // _lib.AyoloError
+decltype(&ayolo_layer_norm_fwd) f_fwd = nullptr;
+decltype(&ayolo_layer_norm_bwd) f_bwd = nullptr;
+decltype(&ayolo_layer_norm_bwd_workspace) f_ws = nullptr;
+decltype(&ayolo_last_error) f_error = nullptr;
+
+struct Refused : std::runtime_error { using std::runtime_error::runtime_error; };
+
+template <typename... A>
+std::string text(const A&... a) { return c10::str(a...); }
+#define REFUSE_UNLESS(cond, ...) do { if (!(cond)) throw Refused(text(__VA_ARGS__)); } while (0)
+
 // equal for tensors of equal shape in equal memory order; dimensions of one element have no order
-uint64_t layout_of(const at::Tensor& t) {
+uint64_t layout_of(const Tensor& t) {
     if (!t.is_non_overlapping_and_dense()) return 0;
     uint64_t h = 1469598103934665603ull;
     for (int64_t d = 0; d < t.dim(); ++d) {
@@ -19,7 +47,7 @@ uint64_t layout_of(const at::Tensor& t) {
     return h | 1;
 }
 
-int dtype_of(const at::Tensor& t) {
+int dtype_of(const Tensor& t) {
     switch (t.scalar_type()) {
         case at::kFloat: return AYOLO_F32;
         case at::kHalf: return AYOLO_F16;
@@ -60,7 +88,7 @@ PyObject* rows(PyObject*, PyObject* args) {
                 ok = false;
             } else {
                 try {
-                    const at::Tensor& t = THPVariable_Unpack(e);
+                    const Tensor& t = THPVariable_Unpack(e);
                     TORCH_CHECK(t.layout() == at::kStrided, "not a strided tensor");
                     row.numel = t.numel();
                     row.dtype = dtype_of(t);
@@ -85,7 +113,240 @@ PyObject* rows(PyObject*, PyObject* args) {
     return out;
 }
 
-PyMethodDef methods[] = {{"rows", rows, METH_VARARGS, "rows(tensors, item=-1) -> bytes of ayolo_tensor"}, {nullptr, nullptr, 0, nullptr}};
+// bump(tensors, given): counts up the version of every tensor of the first list whose entry in the second is not None (kernels
+// write through raw addresses, which autograd's version counters do not see)
+PyObject* bump(PyObject*, PyObject* args) {
+    PyObject *list, *given;
+    if (!PyArg_ParseTuple(args, "O!O!", &PyList_Type, &list, &PyList_Type, &given)) return nullptr;
+    for (Py_ssize_t i = 0; i < PyList_GET_SIZE(list) && i < PyList_GET_SIZE(given); ++i) {
+        PyObject* e = PyList_GET_ITEM(list, i);
+        if (PyList_GET_ITEM(given, i) == Py_None || !THPVariable_Check(e)) continue;
+        const Tensor& t = THPVariable_Unpack(e);
+        if (!t.is_inference()) t.unsafeGetTensorImpl()->bump_version();
+    }
+    Py_RETURN_NONE;
+}
+
+// ------------------------------------------------------------------------------------------------------- layer norm
+// Where the rows (the last dimension) of an operand lie.  Leading dimensions may have any strides that two levels describe (a
+// channel slice of a wider map, a window of a batch of sequences); anything else is copied, and `t` becomes the copy.
+ayolo_rows row_view(Tensor& t) {
+    const int64_t C = t.size(-1);
+    ayolo_rows r{};
+    if (!t.is_contiguous()) {
+        int64_t n[2] = {1, 1}, st[2] = {0, 0};
+        int levels = 0;
+        bool fits = C == 1 || t.stride(-1) == 1;
+        for (int64_t d = t.dim() - 2; d >= 0 && fits; --d) {
+            if (t.size(d) == 1) continue;
+            if (levels > 0 && t.stride(d) == n[levels - 1] * st[levels - 1]) n[levels - 1] *= t.size(d);
+            else if (levels == 2) fits = false;
+            else { n[levels] = t.size(d); st[levels++] = t.stride(d); }
+        }
+        if (fits) {
+            r.data = t.data_ptr();
+            r.stride = levels ? st[0] : C;
+            if (levels == 2) { r.outer_stride = st[1]; r.inner = n[0]; }
+            return r;
+        }
+        t = t.contiguous();
+    }
+    r.data = t.data_ptr();
+    r.stride = C;
+    return r;
+}
+
+void* ptr(const Tensor& t) { return t.defined() ? t.data_ptr() : nullptr; }
+void checked(int rc, const char* what) {
+    if (rc != 0) throw Refused(text(what, " failed (rc=", rc, "): ", f_error()));
+}
+
+// The gain and bias as the kernels read them: both of x's type, or both fp32.
+at::ScalarType params_type(const Tensor& w, const Tensor& b, at::ScalarType dt) {
+    return (w.defined() || b.defined()) && (!w.defined() || w.scalar_type() == dt) && (!b.defined() || b.scalar_type() == dt) ? dt : at::kFloat;
+}
+Tensor as_param(const Tensor& t, at::ScalarType dt) { return t.defined() ? t.detach().to(dt).contiguous() : t; }
+
+struct Norm { Tensor y, s, mean, rstd, w; };
+Norm norm_forward(const Tensor& x0, const Tensor& r0, const Tensor& w0, const Tensor& b0, double eps, int64_t dim, bool stats) {
+    const c10::DeviceGuard guard(x0.device());
+    const at::ScalarType wdt = params_type(w0, b0, x0.scalar_type());
+    const bool last = dim == x0.dim() - 1;
+    Tensor x = last ? x0 : x0.movedim(dim, -1), r = !r0.defined() || last ? r0 : r0.movedim(dim, -1);
+    const int64_t C = x.size(-1), n = x.numel() / C;
+    Norm o;
+    o.w = as_param(w0, wdt);
+    const Tensor b = as_param(b0, wdt);
+    o.y = at::empty(x.sizes(), x.options());
+    if (r.defined()) o.s = at::empty(x.sizes(), x.options());
+    if (stats) {
+        const Tensor both = at::empty({2, n}, x.options().dtype(at::kFloat));
+        o.mean = both.select(0, 0);
+        o.rstd = both.select(0, 1);
+    }
+    const int dt = dtype_of(x);
+    const ayolo_rows xr = row_view(x);
+    ayolo_rows rr{};
+    if (r.defined()) rr = row_view(r);
+    checked(f_fwd(dt, &xr, r.defined() ? &rr : nullptr, n, C, ptr(o.w), ptr(b), wdt == at::kFloat ? AYOLO_F32 : dt, (float)eps, ptr(o.y),
+                  ptr(o.s), (float*)ptr(o.mean), (float*)ptr(o.rstd), c10::hip::getCurrentHIPStream(x.device().index()).stream()),
+            "ayolo_layer_norm_fwd");
+    if (!last) {
+        o.y = o.y.movedim(-1, dim);
+        if (o.s.defined()) o.s = o.s.movedim(-1, dim);
+    }
+    return o;
+}
+
+struct LayerNorm : torch::autograd::Function<LayerNorm> {
+    static variable_list forward(AutogradContext* ctx, const Tensor& x, const std::optional<Tensor>& residual, const std::optional<Tensor>& weight,
+                                 const std::optional<Tensor>& bias, double eps, int64_t dim) {
+        const Tensor r = residual.value_or(Tensor()), w = weight.value_or(Tensor()), b = bias.value_or(Tensor());
+        const Norm o = norm_forward(x, r, w, b, eps, dim, true);
+        ctx->set_materialize_grads(false);
+        ctx->save_for_backward({r.defined() ? o.s : x, o.w, o.mean, o.rstd});
+        auto& kept = ctx->saved_data;
+        kept["dim"] = dim;
+        kept["wtype"] = w.defined() ? (int64_t)w.scalar_type() : -1;
+        kept["btype"] = b.defined() ? (int64_t)b.scalar_type() : -1;
+        kept["ptype"] = (int64_t)params_type(w, b, x.scalar_type());
+        kept["need_x"] = x.requires_grad();
+        kept["need_r"] = r.defined() && r.requires_grad();
+        kept["need_w"] = w.defined() && w.requires_grad();
+        kept["need_b"] = b.defined() && b.requires_grad();
+        if (r.defined()) return {o.y, o.s};
+        return {o.y};
+    }
+
+    static variable_list backward(AutogradContext* ctx, const variable_list& grads) {
+        const variable_list saved = ctx->get_saved_variables();
+        auto& kept = ctx->saved_data;
+        const int64_t dim = kept["dim"].toInt();
+        const bool nx = kept["need_x"].toBool(), nr = kept["need_r"].toBool(), nw = kept["need_w"].toBool(), nb = kept["need_b"].toBool();
+        Tensor s = saved[0], dy = grads[0], q = grads.size() > 1 ? grads[1] : Tensor();
+        Tensor dx, dw, db;
+        if (!dy.defined()) {                               // only the residual sum was used
+            dx = q;
+        } else {
+            const at::NoGradGuard no_grad;
+            const c10::DeviceGuard guard(s.device());
+            const bool last = dim == s.dim() - 1;
+            const at::ScalarType wdt = (at::ScalarType)kept["ptype"].toInt();
+            dy = dy.to(s.scalar_type());
+            if (q.defined()) q = q.to(s.scalar_type());
+            if (!last) {
+                s = s.movedim(dim, -1);
+                dy = dy.movedim(dim, -1);
+                if (q.defined()) q = q.movedim(dim, -1);
+            }
+            const int64_t C = s.size(-1), n = s.numel() / C;
+            const int dt = dtype_of(s);
+            if (nx || nr) dx = at::empty(s.sizes(), s.options());
+            if (nw) dw = at::empty({C}, s.options().dtype(wdt));
+            if (nb) db = at::empty({C}, s.options().dtype(wdt));
+            const size_t need = nw || nb ? f_ws(dt, n, C) : 0;
+            const Tensor ws = need ? at::empty({(int64_t)need}, s.options().dtype(at::kByte)) : Tensor();
+            const ayolo_rows sr = row_view(s), gr = row_view(dy);
+            ayolo_rows qr{};
+            if (q.defined()) qr = row_view(q);
+            checked(f_bwd(dt, &sr, &gr, q.defined() ? &qr : nullptr, n, C, ptr(saved[1]), wdt == at::kFloat ? AYOLO_F32 : dt,
+                          (const float*)ptr(saved[2]), (const float*)ptr(saved[3]), ptr(dx), ptr(dw), ptr(db), ptr(ws), need,
+                          c10::hip::getCurrentHIPStream(s.device().index()).stream()),
+                    "ayolo_layer_norm_bwd");
+            if (!last && dx.defined()) dx = dx.movedim(-1, dim);
+            if (nw) dw = dw.to((at::ScalarType)kept["wtype"].toInt());
+            if (nb) db = db.to((at::ScalarType)kept["btype"].toInt());
+        }
+        variable_list out = {nx ? dx : Tensor(), nr ? dx : Tensor(), dw, db, Tensor(), Tensor()};
+        if (at::GradMode::is_enabled()) {                  // create_graph: what was computed here has no derivative
+            variable_list given;
+            for (int k = 0; k < 4; ++k)
+                if (out[k].defined()) given.push_back(out[k].detach());
+            auto stop = std::make_shared<torch::autograd::DelayedError>("layer_norm is differentiable once", (int)given.size());
+            for (auto& t : given) t.requires_grad_(true);
+            variable_list marked = (*stop)(std::move(given));
+            size_t at = 0;
+            for (int k = 0; k < 4; ++k)
+                if (out[k].defined()) out[k] = marked[at++];
+        }
+        return out;
+    }
+};
+
+// layer_norm(x, weight, bias, eps, residual, dim): y, or (y, x + residual)
+PyObject* layer_norm(PyObject*, PyObject* args) {
+    PyObject *px, *pw, *pb, *pr;
+    double eps;
+    long long dim;
+    if (!PyArg_ParseTuple(args, "OOOdOL", &px, &pw, &pb, &eps, &pr, &dim)) return nullptr;
+    try {
+        auto take = [](PyObject* o, const char* name, bool needed) -> Tensor {
+            if (o == Py_None && !needed) return Tensor();
+            REFUSE_UNLESS(THPVariable_Check(o), "layer_norm: ", name, " is not a tensor");
+            return THPVariable_Unpack(o);
+        };
+        const Tensor x = take(px, "x", true), w = take(pw, "weight", false), b = take(pb, "bias", false), r = take(pr, "residual", false);
+        REFUSE_UNLESS(x.is_cuda(), "layer_norm: the HIP path needs a tensor on the GPU (got ", x.device(), "); there is no CPU fallback");
+        const int dt = dtype_of(x);
+        REFUSE_UNLESS(x.layout() == at::kStrided && dt >= 0 && dt != AYOLO_U8, "layer_norm: unsupported dtype ", x.scalar_type());
+        REFUSE_UNLESS(x.dim() > 0 && -x.dim() <= dim && dim < x.dim(), "layer_norm: no dimension ", dim, " in shape ", x.sizes());
+        if (dim < 0) dim += x.dim();
+        const int64_t C = x.size(dim);
+        REFUSE_UNLESS(C > 0 && C < (1ll << 30) && x.numel() / C < (1ll << 31), "layer_norm: shape ", x.sizes());
+        for (const auto& p : {std::make_pair(&w, "weight"), std::make_pair(&b, "bias")}) {
+            const Tensor& t = *p.first;
+            REFUSE_UNLESS(!t.defined() || (t.dim() == 1 && t.size(0) == C && t.device() == x.device() && t.is_floating_point()),
+                          "layer_norm: ", p.second, " must hold ", C, " floating values on ", x.device());
+        }
+        REFUSE_UNLESS(!r.defined() || (r.sizes() == x.sizes() && r.scalar_type() == x.scalar_type() && r.device() == x.device() && r.layout() == at::kStrided),
+                      "layer_norm: residual must have x's shape ", x.sizes(), ", type ", x.scalar_type(), " and device ", x.device());
+        REFUSE_UNLESS(eps >= 0.0, "layer_norm: eps=", eps);
+        variable_list out;
+        auto grad = [](const Tensor& t) { return t.defined() && t.requires_grad(); };
+        if (at::GradMode::is_enabled() && (grad(x) || grad(r) || grad(w) || grad(b))) {
+            auto opt = [](const Tensor& t) { return t.defined() ? std::optional<Tensor>(t) : std::nullopt; };
+            out = LayerNorm::apply(x, opt(r), opt(w), opt(b), eps, (int64_t)dim);
+        } else {
+            const at::NoGradGuard no_grad;
+            const Norm o = norm_forward(x, r, w, b, eps, dim, false);
+            out.push_back(o.y);
+            if (r.defined()) out.push_back(o.s);
+        }
+        PyObject* y = THPVariable_Wrap(out[0]);
+        if (out.size() == 1 || !y) return y;
+        PyObject* s = THPVariable_Wrap(out[1]);
+        PyObject* both = s ? PyTuple_Pack(2, y, s) : nullptr;
+        Py_DECREF(y);
+        Py_XDECREF(s);
+        return both;
+    } catch (const Refused& e) {
+        PyErr_SetString(ayolo_error ? ayolo_error : PyExc_RuntimeError, e.what());
+    } catch (...) {
+        torch::translate_exception_to_python(std::current_exception());
+    }
+    return nullptr;
+}
+
+// bind(AyoloError, address of ayolo_layer_norm_fwd, _bwd, _bwd_workspace, ayolo_last_error)
+PyObject* bind(PyObject*, PyObject* args) {
+    PyObject* err;
+    unsigned long long a, b, c, d;
+    if (!PyArg_ParseTuple(args, "OKKKK", &err, &a, &b, &c, &d)) return nullptr;
+    Py_INCREF(err);
+    Py_XDECREF(ayolo_error);
+    ayolo_error = err;
+    f_fwd = (decltype(f_fwd))a;
+    f_bwd = (decltype(f_bwd))b;
+    f_ws = (decltype(f_ws))c;
+    f_error = (decltype(f_error))d;
+    Py_RETURN_NONE;
+}
+
+PyMethodDef methods[] = {{"rows", rows, METH_VARARGS, "rows(tensors, item=-1) -> bytes of ayolo_tensor"},
+                         {"bump", bump, METH_VARARGS, "bump(tensors, given): count up the versions of the tensors that are given"},
+                         {"layer_norm", layer_norm, METH_VARARGS, "layer_norm(x, weight, bias, eps, residual, dim)"},
+                         {"bind", bind, METH_VARARGS, "bind(AyoloError, fwd, bwd, bwd_workspace, last_error)"},
+                         {nullptr, nullptr, 0, nullptr}};
 PyModuleDef module = {PyModuleDef_HEAD_INIT, "_host", nullptr, -1, methods, nullptr, nullptr, nullptr, nullptr};
 
 }  // namespace

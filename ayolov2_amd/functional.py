@@ -303,51 +303,6 @@ class Upsample2xFn(torch.autograd.Function):
         return ops.upsample2x_bwd(ops.to_nhwc(dy))
 
 
-def _norm_params(weight, bias, dt: torch.dtype):
-    """The gain and bias as the kernels read them: both of x's type, or both fp32."""
-    ws = [t.detach() for t in (weight, bias) if t is not None]
-    wdt = dt if ws and all(t.dtype == dt for t in ws) else torch.float32
-    conv = [None if t is None else t.detach().to(wdt).contiguous() for t in (weight, bias)]
-    return conv[0], conv[1], wdt
-
-
-class LayerNormFn(torch.autograd.Function):
-    @staticmethod
-    def forward(ctx, x, residual, weight, bias, eps, dim):
-        w, b, wdt = _norm_params(weight, bias, x.dtype)
-        xs = x.movedim(dim, -1)
-        y, s, mean, rstd = ops.layer_norm_fwd(xs, w, b, eps, None if residual is None else residual.movedim(dim, -1), stats=True)
-        y = y.movedim(-1, dim)
-        ctx.set_materialize_grads(False)
-        ctx.dim, ctx.wdt = dim, wdt
-        ctx.wtypes = tuple(None if t is None else t.dtype for t in (weight, bias))
-        if s is None:
-            ctx.save_for_backward(x, w, mean, rstd)
-            return y
-        s = s.movedim(-1, dim)
-        ctx.save_for_backward(s, w, mean, rstd)
-        return y, s
-
-    @staticmethod
-    @torch.autograd.function.once_differentiable
-    def backward(ctx, dy, dsum=None):
-        s, w, mean, rstd = ctx.saved_tensors
-        need_x, need_r, need_w, need_b = ctx.needs_input_grad[:4]
-        if dy is None:                             # only the residual sum was used
-            return (dsum if need_x else None), (dsum if need_r else None), None, None, None, None
-        dim = ctx.dim
-        dx, dw, db = ops.layer_norm_bwd(s.movedim(dim, -1), dy.to(s.dtype).movedim(dim, -1), w, mean, rstd,
-                                        None if dsum is None else dsum.to(s.dtype).movedim(dim, -1), want_dx=need_x or need_r,
-                                        want_dweight=need_w, want_dbias=need_b, wdtype=ctx.wdt)
-        if dx is not None:
-            dx = dx.movedim(-1, dim)
-        if dw is not None:
-            dw = dw.to(ctx.wtypes[0])
-        if db is not None:
-            db = db.to(ctx.wtypes[1])
-        return (dx if need_x else None), (dx if need_r else None), dw, db, None, None
-
-
 def layer_norm(x: torch.Tensor, weight: Optional[torch.Tensor] = None, bias: Optional[torch.Tensor] = None, eps: float = 1e-5,
                residual: Optional[torch.Tensor] = None, dim: int = -1):
     """Layer norm over dimension `dim`: -1 for tokens (..., C), 1 for an activation (B, C, H, W) that lies NHWC in memory.
@@ -358,27 +313,4 @@ def layer_norm(x: torch.Tensor, weight: Optional[torch.Tensor] = None, bias: Opt
     floating, each optional.  Rows may have any strides and any alignment as long as `dim` is contiguous in memory; otherwise x
     is copied first.  Differentiable once, in x, residual, weight and bias; gradients have the inputs' types and the same bits
     in every run."""
-    ops.require_cuda(x, "layer_norm")
-    ops.norm_dtype_code(x.dtype)
-    if x.dim() == 0 or not -x.dim() <= dim < x.dim():
-        raise _lib.AyoloError(f"layer_norm: no dimension {dim} in shape {tuple(x.shape)}")
-    C = x.shape[dim]
-    if C == 0 or x.numel() // C >= 1 << 31:
-        raise _lib.AyoloError(f"layer_norm: shape {tuple(x.shape)}")
-    for t, name in ((weight, "weight"), (bias, "bias")):
-        if t is not None and (t.dim() != 1 or t.shape[0] != C or t.device != x.device or not t.is_floating_point()):
-            raise _lib.AyoloError(f"layer_norm: {name} must hold {C} floating values on {x.device}, got {t.dtype} {tuple(t.shape)} on {t.device}")
-    if residual is not None and (residual.shape != x.shape or residual.dtype != x.dtype or residual.device != x.device):
-        raise _lib.AyoloError(f"layer_norm: residual {residual.dtype} {tuple(residual.shape)} on {residual.device} beside {x.dtype} "
-                              f"{tuple(x.shape)} on {x.device}")
-    if not eps >= 0.0:
-        raise _lib.AyoloError(f"layer_norm: eps={eps}")
-    if torch.is_grad_enabled() and any(t is not None and t.requires_grad for t in (x, residual, weight, bias)):
-        return LayerNormFn.apply(x, residual, weight, bias, eps, dim)
-    w, b, _ = _norm_params(weight, bias, x.dtype)
-    if dim in (-1, x.dim() - 1):
-        y, s, _, _ = ops.layer_norm_fwd(x, w, b, eps, residual)
-    else:
-        y, s, _, _ = ops.layer_norm_fwd(x.movedim(dim, -1), w, b, eps, None if residual is None else residual.movedim(dim, -1))
-        y, s = y.movedim(-1, dim), None if s is None else s.movedim(-1, dim)
-    return y if residual is None else (y, s)
+    return _lib.host().layer_norm(x, weight, bias, float(eps), residual, dim)

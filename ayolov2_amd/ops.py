@@ -339,76 +339,3 @@ def head_grad_pack(draw, dtype: torch.dtype, ldz: int, want_bias=True):
     dbias = torch.zeros(na * no, dtype=torch.float32, device=draw.device) if want_bias else None
     call("ayolo_head_grad_pack", _ptr(draw), B, na, ny, nx, no, dtype_code(dtype), _ptr(dz), ldz, _ptr(dbias), _stream())
     return dz, dbias
-
-
-# --------------------------------------------------------------------------------------------------
-_NORM_DTYPES = {torch.float16: _lib.F16, torch.float32: _lib.F32, torch.bfloat16: _lib.BF16}
-
-
-def norm_dtype_code(dt: torch.dtype) -> int:
-    if dt not in _NORM_DTYPES:
-        raise _lib.AyoloError(f"layer_norm: unsupported dtype {dt}")
-    return _NORM_DTYPES[dt]
-
-
-def row_view(t: torch.Tensor):
-    """(tensor, Rows) of an operand whose rows are its last dimension.  Leading dimensions may have any strides that two levels
-    describe (a channel slice of a wider map, a window of a batch of sequences); anything else is copied."""
-    C = t.shape[-1]
-    if t.is_contiguous():
-        return t, _lib.Rows(t.data_ptr(), C, 0, 0)
-    dims = []                                     # (size, stride) of the leading dimensions, innermost first, merged
-    for n, st in zip(reversed(t.shape[:-1]), reversed(t.stride()[:-1])):
-        if n == 1:
-            continue
-        if dims and st == dims[-1][0] * dims[-1][1]:
-            dims[-1][0] *= n
-        else:
-            dims.append([n, st])
-    if (C > 1 and t.stride(-1) != 1) or len(dims) > 2:
-        t = t.contiguous()
-        return t, _lib.Rows(t.data_ptr(), C, 0, 0)
-    if not dims:
-        return t, _lib.Rows(t.data_ptr(), C, 0, 0)
-    if len(dims) == 1:
-        return t, _lib.Rows(t.data_ptr(), dims[0][1], 0, 0)
-    return t, _lib.Rows(t.data_ptr(), dims[0][1], dims[1][1], dims[0][0])
-
-
-def layer_norm_fwd(x, weight, bias, eps: float, residual=None, stats: bool = False):
-    """Layer norm over the last dimension (ayolo_layer_norm_fwd).  Returns (y, s, mean, rstd): s = x + residual in x's type (None
-    without a residual), mean / rstd fp32 per row (None unless `stats`).  weight / bias: contiguous (C,), fp32 or x's type."""
-    C, dev = x.shape[-1], x.device
-    rows = x.numel() // C
-    y = torch.empty(x.shape, dtype=x.dtype, device=dev)
-    s = torch.empty(x.shape, dtype=x.dtype, device=dev) if residual is not None else None
-    mean = rstd = None
-    if stats:
-        mean, rstd = torch.empty((2, rows), dtype=torch.float32, device=dev).unbind()
-    x, xr = row_view(x)
-    rr = None
-    if residual is not None:
-        residual, rr = row_view(residual)
-    wdt = weight if weight is not None else bias
-    _lib.call_on(x.get_device(), "ayolo_layer_norm_fwd", norm_dtype_code(x.dtype), xr, rr, rows, C, _ptr(weight), _ptr(bias),
-                 norm_dtype_code(wdt.dtype) if wdt is not None else _lib.F32, eps, _ptr(y), _ptr(s), _ptr(mean), _ptr(rstd))
-    return y, s, mean, rstd
-
-
-def layer_norm_bwd(s, dy, weight, mean, rstd, dsum=None, want_dx=True, want_dweight=True, want_dbias=True, wdtype=torch.float32):
-    """Backward of layer_norm_fwd (ayolo_layer_norm_bwd): (dx, dweight, dbias), the parameters' gradients in `wdtype`."""
-    C, dev = s.shape[-1], s.device
-    rows, dt = s.numel() // C, norm_dtype_code(s.dtype)
-    dx = torch.empty(s.shape, dtype=s.dtype, device=dev) if want_dx else None
-    dw = torch.empty(C, dtype=wdtype, device=dev) if want_dweight else None
-    db = torch.empty(C, dtype=wdtype, device=dev) if want_dbias else None
-    need = int(_lib.lib().ayolo_layer_norm_bwd_workspace(dt, rows, C)) if want_dweight or want_dbias else 0
-    ws = torch.empty(need, dtype=torch.uint8, device=dev) if need else None
-    s, sr = row_view(s)
-    dy, gr = row_view(dy)
-    qr = None
-    if dsum is not None:
-        dsum, qr = row_view(dsum)
-    _lib.call_on(s.get_device(), "ayolo_layer_norm_bwd", dt, sr, gr, qr, rows, C, _ptr(weight), norm_dtype_code(wdtype), _ptr(mean),
-                 _ptr(rstd), _ptr(dx), _ptr(dw), _ptr(db), _ptr(ws), need)
-    return dx, dw, db

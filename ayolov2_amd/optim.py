@@ -15,7 +15,6 @@ from __future__ import annotations
 
 import array
 import ctypes
-import math
 from typing import NamedTuple, Optional, Sequence, Tuple, Union
 
 import numpy as np
@@ -212,7 +211,7 @@ def clip_grads_(grads: Sequence[Optional[torch.Tensor]], max_norm: float, norm: 
         norm = grad_norm(grads)
     _lib.call_on(dev.index, "ayolo_grad_clip", _lib.tensor_rows(grads, "clip_grads_"), len(grads), _scalar(norm, dev, "clip_grads_", "norm"),
                  max_norm)
-    _lib.bump_versions(grads)
+    _lib.host().bump(grads, grads)
     return norm
 
 
@@ -257,21 +256,18 @@ def unpack_moments(moments: Sequence[Moment8], signed: bool, out: Optional[Seque
         raise _lib.AyoloError(f"unpack_moments: {len(out)} outputs for {len(moments)} moments")
     _lib.call_on(dev.index, "ayolo_moment_values", _lib.tensor_rows(moments, "unpack_moments", 0), _lib.tensor_rows(moments, "unpack_moments", 1),
                  _lib.tensor_rows(out, "unpack_moments"), len(moments), int(bool(signed)))
-    _lib.bump_versions(out)
+    out = list(out)
+    _lib.host().bump(out, out)
     return out
 
 
 def _per_tensor(v, n: int, what: str):
     """(number, None), or (0, n floats as bytes) where a number per tensor is given."""
     if isinstance(v, (int, float)):
-        if not (math.isfinite(v) and v >= 0.0):
-            raise _lib.AyoloError(f"adamw_step: {what}={v}")
         return float(v), None
     arr = array.array("f", v)
     if len(arr) != n:
         raise _lib.AyoloError(f"adamw_step: {len(arr)} values of {what} for {n} tensors")
-    if not all(0.0 <= x < math.inf for x in arr):
-        raise _lib.AyoloError(f"adamw_step: {what} must be finite and not negative")
     return 0.0, arr.tobytes()
 
 
@@ -300,10 +296,7 @@ def adamw_step(params: Sequence[torch.Tensor], grads: Sequence[Optional[torch.Te
         return
     if (total_norm is None) != (max_norm is None):
         raise _lib.AyoloError("adamw_step: total_norm and max_norm go together")
-    kinds = {isinstance(m, (tuple, list)) for l in (exp_avgs, exp_avg_sqs) for m, g in zip(l, grads) if g is not None}
-    if len(kinds) != 1:
-        raise _lib.AyoloError("adamw_step: moments of 8 and of 32 bits in one call")
-    bits8 = kinds.pop()
+    bits8 = isinstance(next((m for m in exp_avgs if m is not None), None), (tuple, list))      # pairs throughout, or tensors
     rows = _lib.tensor_rows
     L, H = _lib.AdamWList(), _lib.AdamWHyper()
     prows, grows = rows(params, "adamw_step: params"), rows(grads, "adamw_step: grads")
@@ -335,7 +328,7 @@ def adamw_step(params: Sequence[torch.Tensor], grads: Sequence[Optional[torch.Te
     need = int(_lib.lib().ayolo_adamw_workspace(n))
     ws = torch.empty(need, dtype=torch.uint8, device=dev)
     _lib.call_on(dev.index, "ayolo_adamw_step", L, H, ws.data_ptr(), need)
-    _lib.bump_versions(p for p, g in zip(params, grads) if g is not None)         # written through raw pointers
+    _lib.host().bump(params, grads)                # written through raw pointers
 
 
 class AdamW(torch.optim.AdamW):

@@ -252,12 +252,14 @@ def test_adamw_refusals():
     refused("share memory", p=same, m=same)
     refused("memory order", p=torch.zeros(2, 3, 4, 4, device="cuda").contiguous(memory_format=torch.channels_last),
             g=torch.zeros(2, 3, 4, 4, device="cuda"), m=torch.zeros(2, 3, 4, 4, device="cuda"), v=torch.zeros(2, 3, 4, 4, device="cuda"))
-    refused("8 and of 32", m=new_moment8(mk()))
+    refused("not a .codes, exponents. pair", m=new_moment8(mk()))
+    refused("not a tensor", v=new_moment8(mk()))
     refused("exponents", m=tuple(new_moment8(mk(8))), v=(mk(8, torch.uint8), mk(2, torch.uint8)))
     refused("lr=", lr=-1.0)
     refused("lr=", lr=float("nan"))
     refused("2 values of lr", lr=[1.0, 2.0])
-    refused("weight_decay must", weight_decay=[-1.0])
+    refused("weight_decay", weight_decay=[-1.0])
+    refused("lr", lr=[float("inf")])
     refused("betas", betas=(1.0, 0.9))
     refused("eps", eps=-1.0)
     refused("go together", max_norm=1.0)
