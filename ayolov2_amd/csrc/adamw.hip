@@ -53,6 +53,29 @@ template <typename T> __device__ __forceinline__ void store_upto(T* p, float4v v
         if (e < n) p[e] = (T)v[e];
 }
 
+// Four elements at `i` of `n`.  A chunk that lies whole inside its tensor (FULL, a uniform condition) has no guards: a load under
+// a per-lane condition is a branch with a wait behind it, and nothing else would be in flight.
+template <bool FULL> struct At {
+    unsigned i;
+    int left;
+    __device__ __forceinline__ At(unsigned at, int k, unsigned n) {
+        i = at + k * 1024 + threadIdx.x * 4;
+        left = FULL ? 4 : i < n ? (int)min(n - i, 4u) : 0;
+        if (!FULL && i >= n) i = 0;
+    }
+    template <typename T> __device__ __forceinline__ float4v load(const T* p) const { return FULL ? load4(p + i) : load_upto(p + i, left); }
+    template <typename T> __device__ __forceinline__ void store(T* p, float4v v) const {
+        if (FULL) store4(p + i, v);
+        else if (left > 0) store_upto(p + i, v, left);
+    }
+};
+// A whole chunk is four vectors per thread at once; the others go one by one (they are few, and the code stays small).
+template <bool FULL> constexpr int U = FULL ? CHUNK / 1024 : 1;
+template <typename F>
+__device__ __forceinline__ void each_part(unsigned at, unsigned n, F f) {
+    for (unsigned i = at; i < at + CHUNK && i < n; i += 1024) f(i);
+}
+
 // the job whose workgroups hold this one: `first` ascends, so it is the last job with first <= blockIdx.x
 template <typename JOBS>
 __device__ __forceinline__ int find_job(const JOBS& P) {
@@ -77,17 +100,14 @@ struct GJobs {
 };
 static_assert(sizeof(GJobs) <= 4096, "kernel arguments");
 
-template <typename T>
+template <bool FULL, typename T>
 __device__ __forceinline__ double squares(const T* g, unsigned n, unsigned at) {
+    float4v x[U<FULL>];
+#pragma unroll
+    for (int k = 0; k < U<FULL>; ++k) x[k] = At<FULL>(at, k, n).load(g);
     double s = 0.0;
-    float4v x[CHUNK / 1024];
 #pragma unroll
-    for (int k = 0; k < CHUNK / 1024; ++k) {
-        const unsigned i = at + k * 1024 + threadIdx.x * 4;
-        x[k] = load_upto(g + (i < n ? i : 0), i < n ? (int)min(n - i, 4u) : 0);
-    }
-#pragma unroll
-    for (int k = 0; k < CHUNK / 1024; ++k)
+    for (int k = 0; k < U<FULL>; ++k)
 #pragma unroll
         for (int e = 0; e < 4; ++e) s += (double)x[k][e] * (double)x[k][e];
     return s;
@@ -103,9 +123,14 @@ __global__ __launch_bounds__(256) void k_grad_squares(GJobs P) {
     const int j = find_job(P);
     const GJob& J = P.j[j];
     const unsigned at = (blockIdx.x - J.first) * CHUNK;
-    double s = J.dtype == AYOLO_F32   ? squares((const float*)J.g, J.n, at)
-               : J.dtype == AYOLO_F16 ? squares((const half_t*)J.g, J.n, at)
-                                      : squares((const bf16_t*)J.g, J.n, at);
+    const bool full = at + CHUNK <= J.n;
+    auto of = [&](auto* g) {
+        if (full) return squares<true>(g, J.n, at);
+        double t = 0.0;
+        each_part(at, J.n, [&](unsigned i) { t += squares<false>(g, J.n, i); });
+        return t;
+    };
+    double s = J.dtype == AYOLO_F32 ? of((const float*)J.g) : J.dtype == AYOLO_F16 ? of((const half_t*)J.g) : of((const bf16_t*)J.g);
     s = wave_sum(s);
     if ((threadIdx.x & 63) == 0) w[threadIdx.x >> 6] = s;
     __syncthreads();
@@ -132,28 +157,27 @@ __device__ __forceinline__ float clip_factor(const float* norm, float max_norm) 
     return c > 1.0f ? 1.0f : c;
 }
 
-template <typename T>
+template <bool FULL, typename T>
 __device__ __forceinline__ void scale(T* g, unsigned n, unsigned at, float f) {
-    float4v x[CHUNK / 1024];
+    float4v x[U<FULL>];
 #pragma unroll
-    for (int k = 0; k < CHUNK / 1024; ++k) {
-        const unsigned i = at + k * 1024 + threadIdx.x * 4;
-        x[k] = load_upto(g + (i < n ? i : 0), i < n ? (int)min(n - i, 4u) : 0);
-    }
+    for (int k = 0; k < U<FULL>; ++k) x[k] = At<FULL>(at, k, n).load(g);
 #pragma unroll
-    for (int k = 0; k < CHUNK / 1024; ++k) {
-        const unsigned i = at + k * 1024 + threadIdx.x * 4;
-        if (i < n) store_upto(g + i, x[k] * f, (int)min(n - i, 4u));
-    }
+    for (int k = 0; k < U<FULL>; ++k) At<FULL>(at, k, n).store(g, x[k] * f);
 }
 __global__ __launch_bounds__(256) void k_grad_clip(GJobs P) {
     const int j = find_job(P);
     const GJob& J = P.j[j];
     const unsigned at = (blockIdx.x - J.first) * CHUNK;
     const float f = clip_factor(P.norm, P.max_norm);
-    if (J.dtype == AYOLO_F32) scale((float*)J.g, J.n, at, f);
-    else if (J.dtype == AYOLO_F16) scale((half_t*)J.g, J.n, at, f);
-    else scale((bf16_t*)J.g, J.n, at, f);
+    const bool full = at + CHUNK <= J.n;
+    auto of = [&](auto* g) {
+        if (full) scale<true>(g, J.n, at, f);
+        else each_part(at, J.n, [&](unsigned i) { scale<false>(g, J.n, i, f); });
+    };
+    if (J.dtype == AYOLO_F32) of((float*)J.g);
+    else if (J.dtype == AYOLO_F16) of((half_t*)J.g);
+    else of((bf16_t*)J.g);
 }
 
 // -------------------------------------------------------------------------------------------------- 8-bit moments
@@ -180,6 +204,7 @@ __device__ __forceinline__ unsigned mix(unsigned x) {
 }
 constexpr unsigned STRIDE = 0x9E3779B1u;                   // 2^32 / golden ratio, odd
 
+// One code at a time, every value: the way of a wavefront that holds an infinity or a NaN.
 template <bool SIGNED>
 __device__ __forceinline__ float decode(unsigned code, int e) {
     const unsigned mag = SIGNED ? code & 0x7fu : code, top = SIGNED ? 0x7fu : 0xffu;
@@ -194,28 +219,68 @@ __device__ __forceinline__ unsigned encode(float x, int e, unsigned r16) {
     unsigned code = (__float_as_uint(y) + (r16 << 4 | 8u)) >> 20;
     if (!SIGNED && code == 0 && bits != 0) code = 1;
     if (bits >= 0x7f800000u) code = bits == 0x7f800000u ? top - 1 : top;
-    return SIGNED && x < 0.0f ? code | 0x80u : code;
+    return SIGNED && bits <= 0x7f800000u ? code | (__float_as_uint(x) >> 24 & 0x80u) : code;
+}
+// Four codes.  An e4m3 byte is m's code as the hardware's conversion reads it (exponent bias 7), but for the infinity's; v's is
+// put into place as it is.
+template <bool SIGNED>
+__device__ __forceinline__ float4v decode4(unsigned c, int e) {
+    const unsigned high = ((c & 0x7f7f7f7fu) + 0x02020202u) & 0x80808080u;      // the low seven bits of a byte above 0x7d
+    if (__ballot((SIGNED ? high : high & c) != 0)) {
+        return float4v{decode<SIGNED>(c & 255u, e), decode<SIGNED>(c >> 8 & 255u, e), decode<SIGNED>(c >> 16 & 255u, e), decode<SIGNED>(c >> 24, e)};
+    }
+    float4v x;
+    if constexpr (SIGNED) {
+        const auto lo = __builtin_amdgcn_cvt_pk_f32_fp8((int)c, false), hi = __builtin_amdgcn_cvt_pk_f32_fp8((int)c, true);
+        x = float4v{lo[0], lo[1], hi[0], hi[1]};
+        e -= M_BIAS + 127 - 7;
+    } else {
+        x = float4v{__uint_as_float(c << 20 & 0x0ff00000u), __uint_as_float(c << 12 & 0x0ff00000u), __uint_as_float(c << 4 & 0x0ff00000u),
+                    __uint_as_float(c >> 4 & 0x0ff00000u)};
+        e -= V_BIAS;
+    }
+#pragma unroll
+    for (int k = 0; k < 4; ++k) x[k] = __builtin_ldexpf(x[k], e);
+    return x;
 }
 // the largest over the 32 lanes of a block, in all of them
-template <int CTRL> __device__ __forceinline__ int dpp_max(int v) {
-    return max(v, __builtin_amdgcn_update_dpp(0, v, CTRL, 0xf, 0xf, true));
+template <int CTRL> __device__ __forceinline__ unsigned dpp_max(unsigned v) {
+    return max(v, (unsigned)__builtin_amdgcn_update_dpp(0, (int)v, CTRL, 0xf, 0xf, true));
 }
-__device__ __forceinline__ int block_max(int v) {
+__device__ __forceinline__ unsigned block_max(unsigned v) {
     v = dpp_max<0xB1>(v);
     v = dpp_max<0x4E>(v);
     v = dpp_max<0x141>(v);
     v = dpp_max<0x140>(v);
-    const v2u r = __builtin_amdgcn_permlane16_swap((unsigned)v, (unsigned)v, false, false);
-    return max((int)r[0], (int)r[1]);
+    const v2u r = __builtin_amdgcn_permlane16_swap(v, v, false, false);
+    return max(r[0], r[1]);
 }
-__device__ __forceinline__ int block_exponent(float4v x, int least) {
-    int e = least;
+// Four values of a block into codes; `e`: the block's exponent, r: 16 random bits each.
+template <bool SIGNED>
+__device__ __forceinline__ unsigned encode4(float4v x, const unsigned (&r)[4], int& e) {
+    constexpr int BIAS = SIGNED ? M_BIAS : V_BIAS, LEAST = SIGNED ? M_LEAST : V_LEAST;
+    unsigned b[4], top = 0, c = 0;
+#pragma unroll
+    for (int k = 0; k < 4; ++k) top = max(top, b[k] = __float_as_uint(x[k]) & 0x7fffffffu);
+    top = block_max(top);
+    if (__ballot(top >= 0x7f800000u)) {                    // the largest finite one
+        top = 0;
+#pragma unroll
+        for (int k = 0; k < 4; ++k) top = b[k] < 0x7f800000u ? max(top, b[k]) : top;
+        e = max((int)(block_max(top) >> 23), LEAST);
+#pragma unroll
+        for (int k = 0; k < 4; ++k) c |= encode<SIGNED>(x[k], e, r[k]) << 8 * k;
+        return c;
+    }
+    e = max((int)(top >> 23), LEAST);
 #pragma unroll
     for (int k = 0; k < 4; ++k) {
-        const int f = (int)(__float_as_uint(x[k]) >> 23 & 255u);
-        e = f < 255 && f > e ? f : e;
+        unsigned t = (__float_as_uint(__builtin_ldexpf(x[k], BIAS - e)) + (r[k] << 4 | 8u)) >> 20;
+        if constexpr (SIGNED) t = (t & 0x7fu) | (t >> 4 & 0x80u);
+        else t = max(t, min(b[k], 1u));
+        c |= t << 8 * k;
     }
-    return block_max(e);
+    return c;
 }
 __device__ __forceinline__ unsigned load_codes(const uint8_t* p, int n) {
     typedef unsigned u1 __attribute__((aligned(1)));
@@ -233,11 +298,6 @@ __device__ __forceinline__ void store_codes(uint8_t* p, unsigned c, int n) {
     for (int e = 0; e < 3; ++e)
         if (e < n) p[e] = (uint8_t)(c >> 8 * e);
 }
-template <bool SIGNED>
-__device__ __forceinline__ float4v decode4(unsigned c, int e) {
-    return float4v{decode<SIGNED>(c & 255u, e), decode<SIGNED>(c >> 8 & 255u, e), decode<SIGNED>(c >> 16 & 255u, e), decode<SIGNED>(c >> 24, e)};
-}
-
 // ----------------------------------------------------------------------------------------------------------- AdamW
 struct Coef { float step, decay, root; unsigned key; };    // lr / (1 - b1^t), lr wd, 1 / sqrt(1 - b2^t), the tensor's random key
 
@@ -286,25 +346,107 @@ template <bool BITS8> struct AJobs {
 };
 static_assert(sizeof(AJobs<false>) <= 4096 && sizeof(AJobs<true>) <= 4096, "kernel arguments");
 
-struct Scalars { float scale, factor, sign; bool scaled; };
+struct Scalars { float scale, factor; bool scaled; };
 __device__ __forceinline__ float4v true_grad(float4v g, const Scalars& c) {
     if (c.scaled)
 #pragma unroll
         for (int e = 0; e < 4; ++e) g[e] = g[e] / c.scale;
-    return g * (c.sign * c.factor);
+    return g * c.factor;
 }
 // the moments, one rounding per operation (compiled without contraction): a plain sequence of the formula's products and sums
 __device__ __forceinline__ void moments(float4v g, const Hyper& h, float4v& m, float4v& v) {
     m = m * h.b1 + g * h.c1;
     v = v * h.b2 + g * g * h.c2;
 }
+// Square root and quotient by the hardware's own functions, each 1 ulp: with the two roundings around them below 4 u of the
+// step.  They take subnormal arguments for zero, which shows where eps is that small too; then the exact functions are used.
 __device__ __forceinline__ float4v stepped(float4v p, float4v m, float4v v, const Coef& c, float eps) {
+    if (eps >= 1e-18f) {
 #pragma unroll
-    for (int e = 0; e < 4; ++e) {
-        const float d = __builtin_fmaf(sqrtf(v[e]), c.root, eps);
-        p[e] -= __builtin_fmaf(p[e], c.decay, c.step * (m[e] / d));
+        for (int e = 0; e < 4; ++e) {
+            const float d = __builtin_fmaf(__builtin_amdgcn_sqrtf(v[e]), c.root, eps);
+            p[e] -= __builtin_fmaf(p[e], c.decay, c.step * m[e] * __builtin_amdgcn_rcpf(d));
+        }
+    } else {
+#pragma unroll
+        for (int e = 0; e < 4; ++e) {
+            const float d = __builtin_fmaf(sqrtf(v[e]), c.root, eps);
+            p[e] -= __builtin_fmaf(p[e], c.decay, c.step * (m[e] / d));
+        }
     }
     return p;
+}
+
+template <bool FULL, typename T>
+__device__ __forceinline__ void step_chunk(const AJob<false>& J, const Hyper& h, const Coef& c, const Scalars& sc, unsigned at) {
+    T* p = (T*)J.p;
+    const T* g = (const T*)J.g;
+    float4v x[U<FULL>], d[U<FULL>], m[U<FULL>], v[U<FULL>];
+#pragma unroll
+    for (int k = 0; k < U<FULL>; ++k) {
+        const At<FULL> a(at, k, J.n);
+        d[k] = a.load(g);
+        m[k] = a.load(J.m);
+        v[k] = a.load(J.v);
+        x[k] = a.load(p);
+    }
+#pragma unroll
+    for (int k = 0; k < U<FULL>; ++k) {
+        const At<FULL> a(at, k, J.n);
+        moments(true_grad(d[k], sc), h, m[k], v[k]);
+        a.store(J.m, m[k]);
+        a.store(J.v, v[k]);
+        a.store(p, stepped(x[k], m[k], v[k], c, h.eps));
+    }
+}
+// 32 lanes hold one block of 128
+template <bool FULL, typename T>
+__device__ __forceinline__ void step_chunk(const AJob<true>& J, const Hyper& h, const Coef& c, const Scalars& sc, unsigned at) {
+    T* p = (T*)J.p;
+    const T* g = (const T*)J.g;
+    float4v x[U<FULL>], d[U<FULL>];
+    unsigned mc[U<FULL>], vc[U<FULL>];
+    int me[U<FULL>], ve[U<FULL>];
+#pragma unroll
+    for (int k = 0; k < U<FULL>; ++k) {
+        const At<FULL> a(at, k, J.n);
+        d[k] = a.load(g);
+        mc[k] = load_codes(J.m + a.i, a.left);
+        vc[k] = load_codes(J.v + a.i, a.left);
+        me[k] = J.me[a.i / 128];
+        ve[k] = J.ve[a.i / 128];
+        x[k] = a.load(p);
+    }
+#pragma unroll
+    for (int k = 0; k < U<FULL>; ++k) {
+        const At<FULL> a(at, k, J.n);
+        float4v m = decode4<true>(mc[k], me[k]), v = decode4<false>(vc[k], ve[k]);
+        moments(true_grad(d[k], sc), h, m, v);
+        if constexpr (!FULL) {
+#pragma unroll
+            for (int e = 0; e < 4; ++e)                    // past the end: not part of the block
+                if (e >= a.left) m[e] = v[e] = 0.0f;
+        }
+        a.store(p, stepped(x[k], m, v, c, h.eps));
+        unsigned rm[4], rv[4];
+        const unsigned first = (J.origin + a.i) * STRIDE;
+#pragma unroll
+        for (int e = 0; e < 4; ++e) {
+            const unsigned r = mix((first + e * STRIDE) ^ c.key);
+            rm[e] = r >> 16;
+            rv[e] = r & 0xffffu;
+        }
+        int em, ev;
+        const unsigned cm = encode4<true>(m, rm, em), cv = encode4<false>(v, rv, ev);
+        if (FULL || a.left > 0) {
+            store_codes(J.m + a.i, cm, a.left);
+            store_codes(J.v + a.i, cv, a.left);
+            if ((threadIdx.x & 31) == 0) {
+                J.me[a.i / 128] = (uint8_t)em;
+                J.ve[a.i / 128] = (uint8_t)ev;
+            }
+        }
+    }
 }
 
 template <typename T, bool BITS8>
@@ -317,75 +459,10 @@ __global__ __launch_bounds__(256) void k_adamw(AJobs<BITS8> P) {
     Scalars sc;
     sc.scaled = h.grad_scale != nullptr;
     sc.scale = sc.scaled ? *h.grad_scale : 1.0f;
-    sc.factor = h.norm ? clip_factor(h.norm, h.max_norm) : 1.0f;
-    sc.sign = h.maximize ? -1.0f : 1.0f;
+    sc.factor = (h.norm ? clip_factor(h.norm, h.max_norm) : 1.0f) * (h.maximize ? -1.0f : 1.0f);
     const unsigned at = (blockIdx.x - J.first) * CHUNK;
-    T* p = (T*)J.p;
-    const T* g = (const T*)J.g;
-    constexpr int U = CHUNK / 1024;
-    float4v x[U], d[U];
-    int left[U];
-    unsigned pos[U];
-#pragma unroll
-    for (int k = 0; k < U; ++k) {
-        const unsigned i = at + k * 1024 + threadIdx.x * 4;
-        left[k] = i < J.n ? (int)min(J.n - i, 4u) : 0;
-        pos[k] = i < J.n ? i : 0;
-        x[k] = load_upto(p + pos[k], left[k]);
-        d[k] = load_upto(g + pos[k], left[k]);
-    }
-    if constexpr (!BITS8) {
-        float4v m[U], v[U];
-#pragma unroll
-        for (int k = 0; k < U; ++k) {
-            m[k] = load_upto(J.m + pos[k], left[k]);
-            v[k] = load_upto(J.v + pos[k], left[k]);
-        }
-#pragma unroll
-        for (int k = 0; k < U; ++k) {
-            moments(true_grad(d[k], sc), h, m[k], v[k]);
-            if (left[k] > 0) {
-                store_upto(p + pos[k], stepped(x[k], m[k], v[k], c, h.eps), left[k]);
-                store_upto(J.m + pos[k], m[k], left[k]);
-                store_upto(J.v + pos[k], v[k], left[k]);
-            }
-        }
-    } else {
-        unsigned mc[U], vc[U];
-        int me[U], ve[U];
-#pragma unroll
-        for (int k = 0; k < U; ++k) {                      // 32 lanes hold one block of 128
-            mc[k] = load_codes(J.m + pos[k], left[k]);
-            vc[k] = load_codes(J.v + pos[k], left[k]);
-            me[k] = J.me[pos[k] / 128];
-            ve[k] = J.ve[pos[k] / 128];
-        }
-#pragma unroll
-        for (int k = 0; k < U; ++k) {
-            float4v m = decode4<true>(mc[k], me[k]), v = decode4<false>(vc[k], ve[k]);
-            moments(true_grad(d[k], sc), h, m, v);
-#pragma unroll
-            for (int e = 0; e < 4; ++e)                    // past the end: not part of the block
-                if (e >= left[k]) m[e] = v[e] = 0.0f;
-            const int em = block_exponent(m, M_LEAST), ev = block_exponent(v, V_LEAST);
-            if (left[k] > 0) store_upto(p + pos[k], stepped(x[k], m, v, c, h.eps), left[k]);
-            unsigned cm = 0, cv = 0;
-#pragma unroll
-            for (int e = 0; e < 4; ++e) {
-                const unsigned r = mix(((J.origin + pos[k] + e) * STRIDE) ^ c.key);
-                cm |= encode<true>(m[e], em, r >> 16) << 8 * e;
-                cv |= encode<false>(v[e], ev, r & 0xffffu) << 8 * e;
-            }
-            if (left[k] > 0) {
-                store_codes(J.m + pos[k], cm, left[k]);
-                store_codes(J.v + pos[k], cv, left[k]);
-                if ((threadIdx.x & 31) == 0) {
-                    J.me[pos[k] / 128] = (uint8_t)em;
-                    J.ve[pos[k] / 128] = (uint8_t)ev;
-                }
-            }
-        }
-    }
+    if (at + CHUNK <= J.n) step_chunk<true, T>(J, h, c, sc, at);
+    else each_part(at, J.n, [&](unsigned i) { step_chunk<false, T>(J, h, c, sc, i); });
 }
 
 struct UJob { const uint8_t *codes, *exps; float* out; unsigned n, first; };
@@ -395,25 +472,26 @@ struct UJobs {
     UJob j[MAX];
 };
 static_assert(sizeof(UJobs) <= 4096, "kernel arguments");
+template <bool SIGNED, bool FULL>
+__device__ __forceinline__ void values_chunk(const UJob& J, unsigned at) {
+    unsigned c[U<FULL>];
+    int e[U<FULL>];
+#pragma unroll
+    for (int k = 0; k < U<FULL>; ++k) {
+        const At<FULL> a(at, k, J.n);
+        c[k] = load_codes(J.codes + a.i, a.left);
+        e[k] = J.exps[a.i / 128];
+    }
+#pragma unroll
+    for (int k = 0; k < U<FULL>; ++k) At<FULL>(at, k, J.n).store(J.out, decode4<SIGNED>(c[k], e[k]));
+}
 template <bool SIGNED>
 __global__ __launch_bounds__(256) void k_moment_values(UJobs P) {
     const int j = find_job(P);
     const UJob& J = P.j[j];
     const unsigned at = (blockIdx.x - J.first) * CHUNK;
-    constexpr int U = CHUNK / 1024;
-    unsigned c[U];
-    int e[U];
-#pragma unroll
-    for (int k = 0; k < U; ++k) {
-        const unsigned i = at + k * 1024 + threadIdx.x * 4, pos = i < J.n ? i : 0;
-        c[k] = load_codes(J.codes + pos, i < J.n ? (int)min(J.n - i, 4u) : 0);
-        e[k] = J.exps[pos / 128];
-    }
-#pragma unroll
-    for (int k = 0; k < U; ++k) {
-        const unsigned i = at + k * 1024 + threadIdx.x * 4;
-        if (i < J.n) store_upto(J.out + i, decode4<SIGNED>(c[k], e[k]), (int)min(J.n - i, 4u));
-    }
+    if (at + CHUNK <= J.n) values_chunk<SIGNED, true>(J, at);
+    else each_part(at, J.n, [&](unsigned i) { values_chunk<SIGNED, false>(J, i); });
 }
 
 // ------------------------------------------------------------------------------------------------------------- host

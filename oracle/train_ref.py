@@ -72,7 +72,8 @@ def decode(codes, exps, signed: bool):
     codes = np.asarray(codes, dtype=np.uint32)
     mag, top = (codes & 0x7F, 0x7F) if signed else (codes, 0xFF)
     e = np.repeat(np.asarray(exps, dtype=np.int64), BLOCK)[:len(codes)] - (M_BIAS if signed else V_BIAS)
-    x = np.ldexp((mag << 20).astype(np.uint32).view(np.float32).astype(np.float64), e).astype(np.float32)
+    with np.errstate(over="ignore"):
+        x = np.ldexp((mag << 20).astype(np.uint32).view(np.float32).astype(np.float64), e).astype(np.float32)
     x = np.where(mag == top, np.float32(np.nan), np.where(mag == top - 1, np.float32(np.inf), x))
     return np.where(codes & 0x80, -x, x).astype(np.float32) if signed else x.astype(np.float32)
 
@@ -94,5 +95,5 @@ def encode(x, r16, signed: bool):
         code = np.where((code == 0) & (bits != 0), np.uint32(1), code)
     code = np.where(bits == 0x7F800000, top - 1, np.where(bits > 0x7F800000, top, code))
     if signed:
-        code = np.where(x < 0, code | 0x80, code)
+        code = np.where(np.signbit(x) & ~np.isnan(x), code | 0x80, code)
     return code.astype(np.uint8), exps.astype(np.uint8)
