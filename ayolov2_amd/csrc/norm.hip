@@ -28,13 +28,16 @@ template <typename T, int VE> struct Vec { typedef T type __attribute__((ext_vec
 template <typename T> struct Vec<T, 1> { typedef T type; };
 
 template <typename T, int VE>
-__device__ __forceinline__ void load(const T* p, float (&v)[VE]) {
-    const typename Vec<T, VE>::type raw = *reinterpret_cast<const typename Vec<T, VE>::type*>(p);
+__device__ __forceinline__ void widen(const typename Vec<T, VE>::type& raw, float (&v)[VE]) {
     if constexpr (VE == 1) v[0] = (float)raw;
     else {
 #pragma unroll
         for (int e = 0; e < VE; ++e) v[e] = (float)raw[e];
     }
+}
+template <typename T, int VE>
+__device__ __forceinline__ void load(const T* p, float (&v)[VE]) {
+    widen<T, VE>(*reinterpret_cast<const typename Vec<T, VE>::type*>(p), v);
 }
 template <typename T, int VE>
 __device__ __forceinline__ void store(T* p, const float (&v)[VE]) {
@@ -147,69 +150,95 @@ struct Place {
     __device__ __forceinline__ bool own(int e) const { return e >= skip; }
     __device__ __forceinline__ bool any() const { return skip < VE; }
 };
+// A thread's columns, the same in every row.  The smallest team is taken, so that all vectors but the last of each thread lie
+// whole inside the row: only the last has elements to leave out (`mine`: 1 or 0 for each of its elements).
+template <int VE, int TS, int NV>
+struct Columns {
+    int c[NV];
+    bool stores;              // the last vector holds an element of the row
+    float mine[VE];
+    __device__ __forceinline__ Columns(int l, int C) {
+#pragma unroll
+        for (int k = 0; k < NV - 1; ++k) c[k] = (k * TS + l) * VE;
+        const Place<VE> at((NV - 1) * TS + l, C);
+        c[NV - 1] = at.c;
+        stores = at.any();
+#pragma unroll
+        for (int e = 0; e < VE; ++e) mine[e] = at.own(e) ? 1.0f : 0.0f;
+    }
+};
+// 1 / sqrt(x) by the hardware (1 ulp); it takes subnormal arguments for zero, which can be only where eps is that small
+__device__ __forceinline__ float inv_sqrt(float x, float eps) { return eps >= 1e-30f ? __builtin_amdgcn_rsqf(x) : 1.0f / sqrtf(x); }
 
+// Teams walk rows base + team, base + team + step, ...; the next row's loads are issued before the present row is reduced.
 template <typename T, int VE, int TS, int NV, bool RES>
-__global__ __launch_bounds__(TS < 256 ? 256 : TS) void k_ln_fwd(Fwd P) {
+__global__ __launch_bounds__(TS < 128 ? 256 : TS) void k_ln_fwd(Fwd P) {
     constexpr int NT = TS < 128 ? 256 : TS, TEAMS = NT / TS;
+    typedef typename Vec<T, VE>::type V;
     __shared__ float ex[TS > 64 ? 4 * (TS / 64) : 1];
     int phase = 0;
     const int team = threadIdx.x / TS, l = threadIdx.x % TS, C = P.C;
+    const Columns<VE, TS, NV> col(l, C);
     const float inv = 1.0f / (float)C;
     const unsigned step = gridDim.x * TEAMS;
-    for (unsigned base = blockIdx.x * TEAMS; base < P.rows; base += step) {
+    V x[NV], r[RES ? NV : 1];
+    auto fetch = [&](unsigned row) {
+        const T* xr = (const T*)P.x.data + row_at(P.x, row);
+#pragma unroll
+        for (int k = 0; k < NV; ++k) x[k] = *reinterpret_cast<const V*>(xr + col.c[k]);
+        if constexpr (RES) {
+            const T* rr = (const T*)P.r.data + row_at(P.r, row);
+#pragma unroll
+            for (int k = 0; k < NV; ++k) r[k] = *reinterpret_cast<const V*>(rr + col.c[k]);
+        }
+    };
+    unsigned base = blockIdx.x * TEAMS;
+    fetch(min(base + team, P.rows - 1));
+    float w[NV][VE], b[NV][VE];
+#pragma unroll
+    for (int k = 0; k < NV; ++k) {
+        load_param<VE>(P.w, P.wdtype, col.c[k], 1.0f, w[k]);
+        load_param<VE>(P.b, P.wdtype, col.c[k], 0.0f, b[k]);
+    }
+    for (; base < P.rows; base += step) {
         const bool live = base + team < P.rows;            // a team past the last row repeats that row and stores nothing
         const unsigned row = live ? base + team : P.rows - 1;
-        const T* xr = (const T*)P.x.data + row_at(P.x, row);
-        const T* rr = RES ? (const T*)P.r.data + row_at(P.r, row) : nullptr;
         float v[NV][VE];
 #pragma unroll
         for (int k = 0; k < NV; ++k) {
-            const Place<VE> at(k * TS + l, C);
-            load<T, VE>(xr + at.c, v[k]);
-        }
-        if constexpr (RES) {
-            float u[NV][VE];
+            widen<T, VE>(x[k], v[k]);
+            if constexpr (RES) {
+                float u[VE];
+                widen<T, VE>(r[k], u);
 #pragma unroll
-            for (int k = 0; k < NV; ++k) load<T, VE>(rr + Place<VE>(k * TS + l, C).c, u[k]);
-#pragma unroll
-            for (int k = 0; k < NV; ++k) {
-                const Place<VE> at(k * TS + l, C);
-#pragma unroll
-                for (int e = 0; e < VE; ++e) v[k][e] = (float)(T)(v[k][e] + u[k][e]);
-                if (live && at.any()) store<T, VE>((T*)P.s + (int64_t)row * C + at.c, v[k]);
+                for (int e = 0; e < VE; ++e) v[k][e] = (float)(T)(v[k][e] + u[e]);
+                if (live && (k < NV - 1 || col.stores)) store<T, VE>((T*)P.s + (int64_t)row * C + col.c[k], v[k]);
             }
         }
+        if (base + step < P.rows) fetch(min(base + step + team, P.rows - 1));
         float t[1] = {0.0f};
 #pragma unroll
-        for (int k = 0; k < NV; ++k) {
-            const Place<VE> at(k * TS + l, C);
+        for (int k = 0; k < NV; ++k)
 #pragma unroll
-            for (int e = 0; e < VE; ++e) t[0] += at.own(e) ? v[k][e] : 0.0f;
-        }
+            for (int e = 0; e < VE; ++e) t[0] = k < NV - 1 ? t[0] + v[k][e] : __builtin_fmaf(col.mine[e], v[k][e], t[0]);
         team_sum<TS, 1>(t, ex, phase);
         const float mu = t[0] * inv;
         t[0] = 0.0f;
 #pragma unroll
-        for (int k = 0; k < NV; ++k) {
-            const Place<VE> at(k * TS + l, C);
+        for (int k = 0; k < NV; ++k)
 #pragma unroll
             for (int e = 0; e < VE; ++e) {
                 v[k][e] -= mu;
-                t[0] += at.own(e) ? v[k][e] * v[k][e] : 0.0f;
+                t[0] = __builtin_fmaf(k < NV - 1 ? v[k][e] : v[k][e] * col.mine[e], v[k][e], t[0]);
             }
-        }
         team_sum<TS, 1>(t, ex, phase);
-        const float rstd = 1.0f / sqrtf(t[0] * inv + P.eps);
+        const float rstd = inv_sqrt(__builtin_fmaf(t[0], inv, P.eps), P.eps);
         if (live) {
 #pragma unroll
             for (int k = 0; k < NV; ++k) {
-                const Place<VE> at(k * TS + l, C);
-                float w[VE], b[VE];
-                load_param<VE>(P.w, P.wdtype, at.c, 1.0f, w);
-                load_param<VE>(P.b, P.wdtype, at.c, 0.0f, b);
 #pragma unroll
-                for (int e = 0; e < VE; ++e) v[k][e] = __builtin_fmaf(v[k][e] * rstd, w[e], b[e]);
-                if (at.any()) store<T, VE>((T*)P.y + (int64_t)row * C + at.c, v[k]);
+                for (int e = 0; e < VE; ++e) v[k][e] = __builtin_fmaf(v[k][e] * rstd, w[k][e], b[k][e]);
+                if (k < NV - 1 || col.stores) store<T, VE>((T*)P.y + (int64_t)row * C + col.c[k], v[k]);
             }
             if (P.mean && l == 0) {
                 P.mean[row] = mu;
@@ -259,7 +288,7 @@ __global__ __launch_bounds__(1024) void k_ln_fwd_long(Fwd P) {
             for (int e = 0; e < VE; ++e) t[0] += at.own(e) ? (v[e] - mu) * (v[e] - mu) : 0.0f;
         }
         team_sum<1024, 1>(t, ex, phase);
-        const float rstd = 1.0f / sqrtf(t[0] * inv + P.eps);
+        const float rstd = inv_sqrt(__builtin_fmaf(t[0], inv, P.eps), P.eps);
         for (int i = threadIdx.x; i * (int64_t)VE < C; i += 1024) {
             const Place<VE> at(i, C);
             float v[VE], w[VE], b[VE];
@@ -278,52 +307,72 @@ __global__ __launch_bounds__(1024) void k_ln_fwd_long(Fwd P) {
 }
 
 // Backward.  A thread holds the same columns in every row its team walks, so the weight's and the bias's gradients are summed
-// over those rows in its registers; at the end the teams of a workgroup add theirs in LDS, one after the other (a fixed order),
-// and the workgroup writes one line [2][C] of partial sums.  k_ln_params adds the lines.  No atomics: the same call gives the
-// same bits.
+// over those rows in its registers; at the end the teams of a wavefront are added by shuffles, its wavefronts through LDS, in a
+// fixed order, and the workgroup writes one line [2][C] of partial sums.  k_ln_params adds the lines.  No atomics: the same call
+// gives the same bits.
 template <typename T, int VE, int TS, int NV, bool RES>
-__global__ __launch_bounds__(TS < 256 ? 256 : TS) void k_ln_bwd(Bwd P) {
-    constexpr int NT = TS < 128 ? 256 : TS, TEAMS = NT / TS;
+__global__ __launch_bounds__(TS < 128 ? 256 : TS) void k_ln_bwd(Bwd P) {
+    constexpr int NT = TS < 128 ? 256 : TS, TEAMS = NT / TS, CAP = TS * NV * VE;
+    typedef typename Vec<T, VE>::type V;
     __shared__ float ex[TS > 64 ? 4 * (TS / 64) : 1];
-    __shared__ float lines[TS > 64 ? 1 : 2 * TS * NV * VE];
+    __shared__ float lines[TS > 64 ? 1 : 4 * 2 * CAP];
     int phase = 0;
     const int team = threadIdx.x / TS, l = threadIdx.x % TS, C = P.C;
+    const Columns<VE, TS, NV> col(l, C);
     const float inv = 1.0f / (float)C;
     const unsigned step = gridDim.x * TEAMS;
-    float w[NV][VE], dw[NV][VE], db[NV][VE];
+    V x[NV], gy[NV], gs[RES ? NV : 1];
+    float mu, rstd;
+    auto fetch = [&](unsigned row) {
+        const T *sr = (const T*)P.s.data + row_at(P.s, row), *gr = (const T*)P.gy.data + row_at(P.gy, row);
+#pragma unroll
+        for (int k = 0; k < NV; ++k) {
+            x[k] = *reinterpret_cast<const V*>(sr + col.c[k]);
+            gy[k] = *reinterpret_cast<const V*>(gr + col.c[k]);
+        }
+        if constexpr (RES) {
+            const T* qr = (const T*)P.gs.data + row_at(P.gs, row);
+#pragma unroll
+            for (int k = 0; k < NV; ++k) gs[k] = *reinterpret_cast<const V*>(qr + col.c[k]);
+        }
+        mu = P.mean[row];
+        rstd = P.rstd[row];
+    };
+    constexpr bool AHEAD = TS < 1024;                      // 16 wavefronts leave 128 registers each: no room for a second row
+    unsigned base = blockIdx.x * TEAMS;
+    if (AHEAD) fetch(min(base + team, P.rows - 1));
+    float w[NV][VE], own_w[VE], dw[NV][VE], db[NV][VE];
 #pragma unroll
     for (int k = 0; k < NV; ++k) {
-        load_param<VE>(P.w, P.wdtype, Place<VE>(k * TS + l, C).c, 1.0f, w[k]);
+        load_param<VE>(P.w, P.wdtype, col.c[k], 1.0f, w[k]);
 #pragma unroll
         for (int e = 0; e < VE; ++e) dw[k][e] = db[k][e] = 0.0f;
     }
-    for (unsigned base = blockIdx.x * TEAMS; base < P.rows; base += step) {
+#pragma unroll
+    for (int e = 0; e < VE; ++e) own_w[e] = w[NV - 1][e] * col.mine[e];
+    for (; base < P.rows; base += step) {
         const bool live = base + team < P.rows;
         const unsigned row = live ? base + team : P.rows - 1;
-        const T* sr = (const T*)P.s.data + row_at(P.s, row);
-        const T* gr = (const T*)P.gy.data + row_at(P.gy, row);
-        const T* qr = RES ? (const T*)P.gs.data + row_at(P.gs, row) : nullptr;
+        if (!AHEAD) fetch(row);
         float v[NV][VE], g[NV][VE], q[RES ? NV : 1][VE];
+        const float m = mu, s = rstd;
 #pragma unroll
         for (int k = 0; k < NV; ++k) {
-            const Place<VE> at(k * TS + l, C);
-            load<T, VE>(sr + at.c, v[k]);
-            load<T, VE>(gr + at.c, g[k]);
-            if constexpr (RES) load<T, VE>(qr + at.c, q[k]);
+            widen<T, VE>(x[k], v[k]);
+            widen<T, VE>(gy[k], g[k]);
+            if constexpr (RES) widen<T, VE>(gs[k], q[k]);
         }
-        const float mu = P.mean[row], rstd = P.rstd[row];
+        if (AHEAD && base + step < P.rows) fetch(min(base + step + team, P.rows - 1));
         float t[2] = {0.0f, 0.0f};
 #pragma unroll
-        for (int k = 0; k < NV; ++k) {
-            const Place<VE> at(k * TS + l, C);
+        for (int k = 0; k < NV; ++k)
 #pragma unroll
             for (int e = 0; e < VE; ++e) {
-                v[k][e] = (v[k][e] - mu) * rstd;
-                const float gw = at.own(e) ? g[k][e] * w[k][e] : 0.0f;
+                v[k][e] = (v[k][e] - m) * s;
+                const float gw = g[k][e] * (k < NV - 1 ? w[k][e] : own_w[e]);
                 t[0] += gw;
-                t[1] += at.own(e) ? gw * v[k][e] : 0.0f;
+                t[1] = __builtin_fmaf(gw, v[k][e], t[1]);
             }
-        }
         if (live) {
 #pragma unroll
             for (int k = 0; k < NV; ++k)
@@ -338,47 +387,43 @@ __global__ __launch_bounds__(TS < 256 ? 256 : TS) void k_ln_bwd(Bwd P) {
             const float c1 = t[0] * inv, c2 = t[1] * inv;
 #pragma unroll
             for (int k = 0; k < NV; ++k) {
-                const Place<VE> at(k * TS + l, C);
 #pragma unroll
                 for (int e = 0; e < VE; ++e) {
-                    float d = rstd * (__builtin_fmaf(g[k][e], w[k][e], -c1) - v[k][e] * c2);
-                    if constexpr (RES) d += q[k][e];
-                    g[k][e] = d;
+                    const float d = __builtin_fmaf(-v[k][e], c2, __builtin_fmaf(g[k][e], w[k][e], -c1));
+                    g[k][e] = RES ? __builtin_fmaf(s, d, q[RES ? k : 0][e]) : s * d;
                 }
-                if (live && at.any()) store<T, VE>((T*)P.dx + (int64_t)row * C + at.c, g[k]);
+                if (live && (k < NV - 1 || col.stores)) store<T, VE>((T*)P.dx + (int64_t)row * C + col.c[k], g[k]);
             }
         }
     }
     if (!P.part) return;
     float* line = P.part + (int64_t)blockIdx.x * 2 * C;
-    if constexpr (TS > 64) {
+    const Place<VE> last((NV - 1) * TS + l, C);
+    if constexpr (TS < 64) {                               // the wavefront's teams: lanes that hold the same columns
 #pragma unroll
-        for (int k = 0; k < NV; ++k) {
-            const Place<VE> at(k * TS + l, C);
+        for (int k = 0; k < NV; ++k)
 #pragma unroll
             for (int e = 0; e < VE; ++e)
-                if (at.own(e)) {
-                    line[at.c + e] = dw[k][e];
-                    line[C + at.c + e] = db[k][e];
-                }
-        }
-    } else {
-        for (int n = 0; n < TEAMS; ++n) {
-            if (team == n) {
 #pragma unroll
-                for (int k = 0; k < NV; ++k) {
-                    const Place<VE> at(k * TS + l, C);
-#pragma unroll
-                    for (int e = 0; e < VE; ++e)
-                        if (at.own(e)) {
-                            lines[at.c + e] = (n ? lines[at.c + e] : 0.0f) + dw[k][e];
-                            lines[C + at.c + e] = (n ? lines[C + at.c + e] : 0.0f) + db[k][e];
-                        }
+                for (int d = TS; d < 64; d *= 2) {
+                    dw[k][e] += __shfl_xor(dw[k][e], d);
+                    db[k][e] += __shfl_xor(db[k][e], d);
                 }
-            }
-            __syncthreads();
-        }
-        for (int i = threadIdx.x; i < 2 * C; i += NT) line[i] = lines[i];
+    }
+    float* to = TS > 64 ? line : lines + (threadIdx.x >> 6) * 2 * C;
+    if (TS >= 64 || (threadIdx.x & 63) < TS) {
+#pragma unroll
+        for (int k = 0; k < NV; ++k)
+#pragma unroll
+            for (int e = 0; e < VE; ++e)
+                if (k < NV - 1 || last.own(e)) {
+                    to[col.c[k] + e] = dw[k][e];
+                    to[C + col.c[k] + e] = db[k][e];
+                }
+    }
+    if constexpr (TS <= 64) {
+        __syncthreads();
+        for (int i = threadIdx.x; i < 2 * C; i += NT) line[i] = (lines[i] + lines[2 * C + i]) + (lines[4 * C + i] + lines[6 * C + i]);
     }
 }
 
@@ -452,10 +497,11 @@ __global__ __launch_bounds__(1024) void k_ln_params(const float* part, int n, in
     float t = 0.0f;
     if (i < 2 * (int64_t)C) {
         int k = slice;
-        for (; k + 96 < n; k += 128) {                     // four loads in flight
-            const float a = part[(int64_t)k * 2 * C + i], b = part[(int64_t)(k + 32) * 2 * C + i];
-            const float d = part[(int64_t)(k + 64) * 2 * C + i], e = part[(int64_t)(k + 96) * 2 * C + i];
-            t += (a + b) + (d + e);
+        for (; k + 7 * 32 < n; k += 8 * 32) {              // eight loads in flight
+            float v[8];
+#pragma unroll
+            for (int u = 0; u < 8; ++u) v[u] = part[(int64_t)(k + 32 * u) * 2 * C + i];
+            t += ((v[0] + v[1]) + (v[2] + v[3])) + ((v[4] + v[5]) + (v[6] + v[7]));
         }
         for (; k < n; k += 32) t += part[(int64_t)k * 2 * C + i];
     }
@@ -489,15 +535,28 @@ Team team_of(int64_t nvec) {
 int ve_of(int dtype, int C) { const int ve = dtype == AYOLO_F32 ? 4 : 8; return C < ve ? 1 : ve; }
 int rows_per_wg(const Team& t) { return t.ts == 0 || t.ts >= 128 ? 1 : 256 / t.ts; }
 
-// workgroups of the backward pass (= lines of partial sums): enough to fill the CUs, few enough that the lines (8 C bytes each,
-// written and read) stay small beside the rows
+int threads_of(const Team& t) { return t.ts < 128 ? 256 : t.ts; }
+
+// Workgroups of the backward pass (= lines of partial sums): eight wavefronts per CU.  Each writes and k_ln_params reads a line
+// of 8 C bytes, and its rows are prefetched, so more wavefronts cost more than they hide: 16384 x 4096 bf16 takes 114 / 87 / 102 /
+// 120 us with 4 / 8 / 16 / 32 of them, 4096 x 8192 bf16 47 / 58 / 85 us with 8 / 16 / 32, 30000 x 640 fp32 66 / 48 / 48 us with
+// 4 / 8 / 16.  And six rows a line, so that the lines stay below the rows' own bytes: 3001 x 1023 fp32 takes 13 us with 512 lines
+// and 16 us with 1024.
 int bwd_groups(int dtype, int64_t rows, int C) {
     const Team t = team_of(cdiv64(C, ve_of(dtype, C)));
     if (t.ts == 0) return (int)(rows < 64 ? rows : 64);
-    const int64_t need = cdiv64(rows, rows_per_wg(t));
-    const int per_cu = t.ts <= 128 ? 4 : t.ts == 256 ? 2 : 1;
-    const int64_t most = (int64_t)cus() * per_cu;
-    return (int)(need < most ? need : most);
+    int64_t n = cdiv64(rows, rows_per_wg(t));
+    const int64_t nt = threads_of(t), most = (int64_t)cus() * (nt < 512 ? 512 / nt : 1), few = rows / 6 > 64 ? rows / 6 : 64;
+    if (n > most) n = most;
+    return (int)(n < few ? n : few);
+}
+
+// Workgroups of the forward pass: what the CUs hold at once (2048 threads each), so that a team walks several rows with its gain
+// and bias in registers; up to twice that every team has one row, which spreads better than one or two (25600 x 256 fp16: 7.6
+// against 8.3 us).
+int64_t fwd_groups(int64_t rows, const Team& t) {
+    const int64_t need = cdiv64(rows, rows_per_wg(t)), most = (int64_t)cus() * (2048 / threads_of(t));
+    return need <= 2 * most ? need : most;
 }
 
 template <typename T, int VE, bool RES>
@@ -506,10 +565,9 @@ void run_fwd(const Fwd& P, const Team& t, hipStream_t s) {
         hipLaunchKernelGGL((k_ln_fwd_long<T, VE, RES>), dim3(P.rows < 65536u ? P.rows : 65536u), dim3(1024), 0, s, P);
         return;
     }
-    const int64_t need = cdiv64(P.rows, rows_per_wg(t)), most = (int64_t)cus() * 64;
-    const dim3 grid((unsigned)(need < most ? need : most));
+    const dim3 grid((unsigned)fwd_groups(P.rows, t));
 #define AY_LN(TS_, NV_) \
-    if (t.ts == TS_ && t.nv == NV_) hipLaunchKernelGGL((k_ln_fwd<T, VE, TS_, NV_, RES>), grid, dim3(TS_ < 128 ? 256 : TS_), 0, s, P)
+    if (t.ts == TS_ && t.nv == NV_) hipLaunchKernelGGL((k_ln_fwd<T, VE, TS_, NV_, RES>), grid, dim3(threads_of(t)), 0, s, P)
     if constexpr (VE == 1) { AY_LN(4, 1); AY_LN(8, 1); }
     else { AY_LN(4, 1); AY_LN(8, 1); AY_LN(16, 1); AY_LN(32, 1); AY_LN(64, 1); AY_LN(64, 2); AY_LN(128, 2); AY_LN(256, 2); AY_LN(512, 2); AY_LN(1024, 2); }
 #undef AY_LN
@@ -523,7 +581,7 @@ void run_bwd(const Bwd& P, const Team& t, int groups, hipStream_t s) {
     }
     const dim3 grid((unsigned)groups);
 #define AY_LN(TS_, NV_) \
-    if (t.ts == TS_ && t.nv == NV_) hipLaunchKernelGGL((k_ln_bwd<T, VE, TS_, NV_, RES>), grid, dim3(TS_ < 128 ? 256 : TS_), 0, s, P)
+    if (t.ts == TS_ && t.nv == NV_) hipLaunchKernelGGL((k_ln_bwd<T, VE, TS_, NV_, RES>), grid, dim3(threads_of(t)), 0, s, P)
     if constexpr (VE == 1) { AY_LN(4, 1); AY_LN(8, 1); }
     else { AY_LN(4, 1); AY_LN(8, 1); AY_LN(16, 1); AY_LN(32, 1); AY_LN(64, 1); AY_LN(64, 2); AY_LN(128, 2); AY_LN(256, 2); AY_LN(512, 2); AY_LN(1024, 2); }
 #undef AY_LN
