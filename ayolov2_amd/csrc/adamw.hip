@@ -7,10 +7,11 @@
 //   p -= lr wd p + lr / (1 - b1^t) * m / (sqrt(v) / sqrt(1 - b2^t) + eps)
 //
 // Bound: HBM.  Per fp32 parameter 4 B for the norm, 8 B for the clipping, 28 B for AdamW with 32-bit moments and 16 B with 8-bit
-// ones.  The tensors come as a list on the host and travel BY VALUE in the kernel arguments (up to 4 KB per launch: some 80
-// tensors), so nothing is copied to the device, nothing has to be kept between calls, and a captured call replays as it is.
-// A workgroup takes CHUNK elements of one tensor; it finds its tensor with one vector compare and a ballot over the jobs'
-// first workgroups.
+// ones.  The tensors come as a list on the host and travel BY VALUE in the kernel arguments (up to 4 KB per launch), so nothing is
+// copied to the device, nothing has to be kept between calls, and a captured call replays as it is.  An address is kept as a
+// 32-bit distance from the launch's first tensor, so that a launch takes 330 gradients, 160 tensors with 32-bit and 120 with 8-bit
+// moments: every further launch costs some 4 us of start and drain.
+// A workgroup takes CHUNK elements of one tensor; it finds its tensor by comparing the jobs' first workgroups 64 at a time.
 #include "common.h"
 #include <math.h>
 #include <algorithm>
@@ -24,7 +25,7 @@ namespace {
 
 constexpr int CHUNK = 4096;                                // elements per workgroup: 256 threads x 4 vectors of 4
 constexpr unsigned PART = 1u << 30;                        // a larger tensor travels as several jobs (a multiple of CHUNK)
-constexpr unsigned MOST_WGS = 1u << 22;                    // of a launch, before its last job (at most 2^18 more): far below 2^32 threads
+constexpr unsigned MOST_WGS = 1u << 20;                    // of a launch, before its last job (at most 2^18 more)
 
 template <typename T> struct V4 { typedef T type __attribute__((ext_vector_type(4), aligned(sizeof(T)))); };
 template <typename T> __device__ __forceinline__ float4v load4(const T* p) {
@@ -76,28 +77,42 @@ __device__ __forceinline__ void each_part(unsigned at, unsigned n, F f) {
     for (unsigned i = at; i < at + CHUNK && i < n; i += 1024) f(i);
 }
 
-// the job whose workgroups hold this one: `first` ascends, so it is the last job with first <= blockIdx.x
-template <typename JOBS>
-__device__ __forceinline__ int find_job(const JOBS& P) {
-    int j = 0;
-    for (int base = 0; base < P.njobs; base += 64) {
-        const int i = base + (int)(threadIdx.x & 63);
-        const bool below = i < P.njobs && P.j[i < P.njobs ? i : 0].first <= blockIdx.x;
-        j += __popcll(__ballot(below));
+// A launch's tensors.  HEAD: what the kernel needs besides; N addresses per tensor, each in steps of its own unit.
+struct Where { unsigned first, tag, tensor; };             // first workgroup; two bits of the caller's; place in the caller's list
+template <typename HEAD, int N> struct Jobs {
+    static constexpr int ADDRESSES = N;
+    struct Job {
+        int off[N];
+        unsigned n, meta;                                  // elements; first workgroup (21 bits), tag (2), place (9)
+    };
+    static constexpr int MAX = (4096 - (int)sizeof(HEAD) - 8 * N - 16) / (int)sizeof(Job);
+    HEAD h;
+    char* base[N];
+    int njobs;
+    unsigned tensor0;
+    Job j[MAX];
+    template <typename T> __device__ __forceinline__ T* at(int k, int a, int unit = sizeof(T)) const { return (T*)(base[a] + (int64_t)j[k].off[a] * unit); }
+    __device__ __forceinline__ Where where(int k) const {
+        const unsigned m = j[k].meta;
+        return Where{m & 0x1fffffu, m >> 21 & 3u, tensor0 + (m >> 23)};
     }
-    return __builtin_amdgcn_readfirstlane(j - 1);
-}
+    // the job whose workgroups hold this one (`first` ascends): every `s`-th job first, then the ones behind it
+    __device__ __forceinline__ int mine() const {
+        const int lane = (int)(threadIdx.x & 63), s = (njobs + 63) / 64;
+        auto below = [&](int i, bool ask) { return __popcll(__ballot(ask && (j[ask ? i : 0].meta & 0x1fffffu) <= blockIdx.x)); };
+        int k = (below(lane * s, lane * s < njobs) - 1) * s;
+        if (s > 1) k += below(k + lane, lane < s && k + lane < njobs) - 1;
+        return __builtin_amdgcn_readfirstlane(k);
+    }
+};
 
 // ------------------------------------------------------------------------------------------------ norm and clipping
-struct GJob { void* g; unsigned n, first; int dtype, pad; };
-struct GJobs {
-    static constexpr int MAX = 160;
+struct GHead {
     const float* norm;
     double* part;
     float max_norm;
-    int njobs;
-    GJob j[MAX];
 };
+typedef Jobs<GHead, 1> GJobs;                              // tag: the gradient's type; unit: 2 bytes
 static_assert(sizeof(GJobs) <= 4096, "kernel arguments");
 
 template <bool FULL, typename T>
@@ -120,21 +135,22 @@ __device__ __forceinline__ double wave_sum(double v) {
 // does not show in the rounded result.  fp64 runs at half the fp32 rate here and stays far below the memory time.
 __global__ __launch_bounds__(256) void k_grad_squares(GJobs P) {
     __shared__ double w[4];
-    const int j = find_job(P);
-    const GJob& J = P.j[j];
-    const unsigned at = (blockIdx.x - J.first) * CHUNK;
-    const bool full = at + CHUNK <= J.n;
+    const int j = P.mine();
+    const Where J = P.where(j);
+    const unsigned at = (blockIdx.x - J.first) * CHUNK, n = P.j[j].n;
     auto of = [&](auto* g) {
-        if (full) return squares<true>(g, J.n, at);
+        if (at + CHUNK <= n) return squares<true>(g, n, at);
         double t = 0.0;
-        each_part(at, J.n, [&](unsigned i) { t += squares<false>(g, J.n, i); });
+        each_part(at, n, [&](unsigned i) { t += squares<false>(g, n, i); });
         return t;
     };
-    double s = J.dtype == AYOLO_F32 ? of((const float*)J.g) : J.dtype == AYOLO_F16 ? of((const half_t*)J.g) : of((const bf16_t*)J.g);
+    double s = J.tag == AYOLO_F32   ? of(P.at<const float>(j, 0, 2))
+               : J.tag == AYOLO_F16 ? of(P.at<const half_t>(j, 0, 2))
+                                    : of(P.at<const bf16_t>(j, 0, 2));
     s = wave_sum(s);
     if ((threadIdx.x & 63) == 0) w[threadIdx.x >> 6] = s;
     __syncthreads();
-    if (threadIdx.x == 0) P.part[blockIdx.x] = (w[0] + w[1]) + (w[2] + w[3]);
+    if (threadIdx.x == 0) P.h.part[blockIdx.x] = (w[0] + w[1]) + (w[2] + w[3]);
 }
 __global__ __launch_bounds__(1024) void k_grad_norm(const double* part, int64_t n, const float* grad_scale, float* out) {
     __shared__ double w[16];
@@ -166,18 +182,17 @@ __device__ __forceinline__ void scale(T* g, unsigned n, unsigned at, float f) {
     for (int k = 0; k < U<FULL>; ++k) At<FULL>(at, k, n).store(g, x[k] * f);
 }
 __global__ __launch_bounds__(256) void k_grad_clip(GJobs P) {
-    const int j = find_job(P);
-    const GJob& J = P.j[j];
-    const unsigned at = (blockIdx.x - J.first) * CHUNK;
-    const float f = clip_factor(P.norm, P.max_norm);
-    const bool full = at + CHUNK <= J.n;
+    const int j = P.mine();
+    const Where J = P.where(j);
+    const unsigned at = (blockIdx.x - J.first) * CHUNK, n = P.j[j].n;
+    const float f = clip_factor(P.h.norm, P.h.max_norm);
     auto of = [&](auto* g) {
-        if (full) scale<true>(g, J.n, at, f);
-        else each_part(at, J.n, [&](unsigned i) { scale<false>(g, J.n, i, f); });
+        if (at + CHUNK <= n) scale<true>(g, n, at, f);
+        else each_part(at, n, [&](unsigned i) { scale<false>(g, n, i, f); });
     };
-    if (J.dtype == AYOLO_F32) of((float*)J.g);
-    else if (J.dtype == AYOLO_F16) of((half_t*)J.g);
-    else of((bf16_t*)J.g);
+    if (J.tag == AYOLO_F32) of(P.at<float>(j, 0, 2));
+    else if (J.tag == AYOLO_F16) of(P.at<half_t>(j, 0, 2));
+    else of(P.at<bf16_t>(j, 0, 2));
 }
 
 // -------------------------------------------------------------------------------------------------- 8-bit moments
@@ -301,32 +316,37 @@ __device__ __forceinline__ void store_codes(uint8_t* p, unsigned c, int n) {
 // ----------------------------------------------------------------------------------------------------------- AdamW
 struct Coef { float step, decay, root; unsigned key; };    // lr / (1 - b1^t), lr wd, 1 / sqrt(1 - b2^t), the tensor's random key
 
+// Tensors that share a learning rate and decay share an entry of `pair`.
 struct PrepJobs {
-    static constexpr int MAX = 240;
+    static constexpr int MAX = 430, PAIRS = 64;
     double ln_b1, ln_b2;
     const float *lr, *found_inf;
     Coef* out;
-    unsigned seed;
-    int n, base, pad;
-    struct { float* step; float lr, wd; } j[MAX];
+    char* step;
+    unsigned seed, place0;
+    int n, pairs;
+    struct { float lr, wd; } pair[PAIRS];
+    struct { int off; unsigned which; } j[MAX];            // the step count's place; pair (6 bits), place in the list - place0 (26)
 };
 static_assert(sizeof(PrepJobs) <= 4096, "kernel arguments");
 
 // One thread per tensor: count the step and leave what depends on it to the update kernels.  1 - b^t in fp64: for b = 0.999 and
 // the first steps an fp32 difference would keep few of its bits.
-__global__ __launch_bounds__(256) void k_adamw_prepare(PrepJobs P) {
+__global__ __launch_bounds__(512) void k_adamw_prepare(PrepJobs P) {
     const int i = threadIdx.x;
-    if (i >= P.n || !P.j[i].step) return;
+    if (i >= P.n) return;
     if (P.found_inf && *P.found_inf != 0.0f) return;
-    const float t = *P.j[i].step + 1.0f;
-    *P.j[i].step = t;
-    const double lr = P.lr ? (double)*P.lr : (double)P.j[i].lr;
+    float* step = (float*)(P.step + (int64_t)P.j[i].off * 4);
+    const unsigned pair = P.j[i].which & 63u, place = P.place0 + (P.j[i].which >> 6);
+    const float t = *step + 1.0f;
+    *step = t;
+    const double lr = P.lr ? (double)*P.lr : (double)P.pair[pair].lr;
     Coef c;
     c.step = (float)(lr / -expm1((double)t * P.ln_b1));
-    c.decay = (float)(lr * (double)P.j[i].wd);
+    c.decay = (float)(lr * (double)P.pair[pair].wd);
     c.root = (float)(1.0 / sqrt(-expm1((double)t * P.ln_b2)));
-    c.key = mix(mix(P.seed + STRIDE * (unsigned)t) + STRIDE * (unsigned)(P.base + i + 1));
-    P.out[P.base + i] = c;
+    c.key = mix(mix(P.seed + STRIDE * (unsigned)t) + STRIDE * (place + 1));
+    P.out[place] = c;
 }
 
 struct Hyper {
@@ -335,16 +355,26 @@ struct Hyper {
     float b1, c1, b2, c2, eps, max_norm;
     int maximize;
 };
-template <bool BITS8> struct AJob;
-template <> struct AJob<false> { void* p; const void* g; float *m, *v; unsigned n, first, tensor, origin; };
-template <> struct AJob<true> { void* p; const void* g; uint8_t *m, *v, *me, *ve; unsigned n, first, tensor, origin; };
-template <bool BITS8> struct AJobs {
-    static constexpr int MAX = BITS8 ? 60 : 80;
-    Hyper h;
-    int njobs, pad;
-    AJob<BITS8> j[MAX];
-};
+// p, g, m, v (and the moments' exponents); tag: which 2^30 elements of its tensor a job is
+template <bool BITS8> using AJobs = Jobs<Hyper, BITS8 ? 6 : 4>;
 static_assert(sizeof(AJobs<false>) <= 4096 && sizeof(AJobs<true>) <= 4096, "kernel arguments");
+template <typename T, bool BITS8> struct Tensor;
+template <typename T> struct Tensor<T, false> {
+    T* p;
+    const T* g;
+    float *m, *v;
+    unsigned n, origin;
+    __device__ __forceinline__ Tensor(const AJobs<false>& P, int j) : p(P.template at<T>(j, 0)), g(P.template at<const T>(j, 1)), m(P.template at<float>(j, 2)), v(P.template at<float>(j, 3)), n(P.j[j].n), origin(0) {}
+};
+template <typename T> struct Tensor<T, true> {
+    T* p;
+    const T* g;
+    uint8_t *m, *v, *me, *ve;
+    unsigned n, origin;                                    // origin: the job's first element in its tensor
+    __device__ __forceinline__ Tensor(const AJobs<true>& P, int j)
+        : p(P.template at<T>(j, 0)), g(P.template at<const T>(j, 1)), m(P.template at<uint8_t>(j, 2)), v(P.template at<uint8_t>(j, 3)),
+          me(P.template at<uint8_t>(j, 4)), ve(P.template at<uint8_t>(j, 5)), n(P.j[j].n), origin(P.where(j).tag * PART) {}
+};
 
 struct Scalars { float scale, factor; bool scaled; };
 __device__ __forceinline__ float4v true_grad(float4v g, const Scalars& c) {
@@ -378,17 +408,15 @@ __device__ __forceinline__ float4v stepped(float4v p, float4v m, float4v v, cons
 }
 
 template <bool FULL, typename T>
-__device__ __forceinline__ void step_chunk(const AJob<false>& J, const Hyper& h, const Coef& c, const Scalars& sc, unsigned at) {
-    T* p = (T*)J.p;
-    const T* g = (const T*)J.g;
+__device__ __forceinline__ void step_chunk(const Tensor<T, false>& J, const Hyper& h, const Coef& c, const Scalars& sc, unsigned at) {
     float4v x[U<FULL>], d[U<FULL>], m[U<FULL>], v[U<FULL>];
 #pragma unroll
     for (int k = 0; k < U<FULL>; ++k) {
         const At<FULL> a(at, k, J.n);
-        d[k] = a.load(g);
+        d[k] = a.load(J.g);
         m[k] = a.load(J.m);
         v[k] = a.load(J.v);
-        x[k] = a.load(p);
+        x[k] = a.load(J.p);
     }
 #pragma unroll
     for (int k = 0; k < U<FULL>; ++k) {
@@ -396,26 +424,24 @@ __device__ __forceinline__ void step_chunk(const AJob<false>& J, const Hyper& h,
         moments(true_grad(d[k], sc), h, m[k], v[k]);
         a.store(J.m, m[k]);
         a.store(J.v, v[k]);
-        a.store(p, stepped(x[k], m[k], v[k], c, h.eps));
+        a.store(J.p, stepped(x[k], m[k], v[k], c, h.eps));
     }
 }
 // 32 lanes hold one block of 128
 template <bool FULL, typename T>
-__device__ __forceinline__ void step_chunk(const AJob<true>& J, const Hyper& h, const Coef& c, const Scalars& sc, unsigned at) {
-    T* p = (T*)J.p;
-    const T* g = (const T*)J.g;
+__device__ __forceinline__ void step_chunk(const Tensor<T, true>& J, const Hyper& h, const Coef& c, const Scalars& sc, unsigned at) {
     float4v x[U<FULL>], d[U<FULL>];
     unsigned mc[U<FULL>], vc[U<FULL>];
     int me[U<FULL>], ve[U<FULL>];
 #pragma unroll
     for (int k = 0; k < U<FULL>; ++k) {
         const At<FULL> a(at, k, J.n);
-        d[k] = a.load(g);
+        d[k] = a.load(J.g);
         mc[k] = load_codes(J.m + a.i, a.left);
         vc[k] = load_codes(J.v + a.i, a.left);
         me[k] = J.me[a.i / 128];
         ve[k] = J.ve[a.i / 128];
-        x[k] = a.load(p);
+        x[k] = a.load(J.p);
     }
 #pragma unroll
     for (int k = 0; k < U<FULL>; ++k) {
@@ -427,7 +453,7 @@ __device__ __forceinline__ void step_chunk(const AJob<true>& J, const Hyper& h, 
             for (int e = 0; e < 4; ++e)                    // past the end: not part of the block
                 if (e >= a.left) m[e] = v[e] = 0.0f;
         }
-        a.store(p, stepped(x[k], m, v, c, h.eps));
+        a.store(J.p, stepped(x[k], m, v, c, h.eps));
         unsigned rm[4], rv[4];
         const unsigned first = (J.origin + a.i) * STRIDE;
 #pragma unroll
@@ -453,45 +479,43 @@ template <typename T, bool BITS8>
 __global__ __launch_bounds__(256) void k_adamw(AJobs<BITS8> P) {
     const Hyper& h = P.h;
     if (h.found_inf && *h.found_inf != 0.0f) return;
-    const int j = find_job(P);
-    const AJob<BITS8>& J = P.j[j];
-    const Coef c = h.coef[J.tensor];
+    const int j = P.mine();
+    const Where W = P.where(j);
+    const Tensor<T, BITS8> J(P, j);
+    const Coef c = h.coef[W.tensor];
     Scalars sc;
     sc.scaled = h.grad_scale != nullptr;
     sc.scale = sc.scaled ? *h.grad_scale : 1.0f;
     sc.factor = (h.norm ? clip_factor(h.norm, h.max_norm) : 1.0f) * (h.maximize ? -1.0f : 1.0f);
-    const unsigned at = (blockIdx.x - J.first) * CHUNK;
-    if (at + CHUNK <= J.n) step_chunk<true, T>(J, h, c, sc, at);
-    else each_part(at, J.n, [&](unsigned i) { step_chunk<false, T>(J, h, c, sc, i); });
+    const unsigned at = (blockIdx.x - W.first) * CHUNK;
+    if (at + CHUNK <= J.n) step_chunk<true>(J, h, c, sc, at);
+    else each_part(at, J.n, [&](unsigned i) { step_chunk<false>(J, h, c, sc, i); });
 }
 
-struct UJob { const uint8_t *codes, *exps; float* out; unsigned n, first; };
-struct UJobs {
-    static constexpr int MAX = 120;
-    int njobs, pad;
-    UJob j[MAX];
-};
+struct None {};
+typedef Jobs<None, 3> UJobs;                               // codes, exponents, values
 static_assert(sizeof(UJobs) <= 4096, "kernel arguments");
 template <bool SIGNED, bool FULL>
-__device__ __forceinline__ void values_chunk(const UJob& J, unsigned at) {
+__device__ __forceinline__ void values_chunk(const uint8_t* codes, const uint8_t* exps, float* out, unsigned n, unsigned at) {
     unsigned c[U<FULL>];
     int e[U<FULL>];
 #pragma unroll
     for (int k = 0; k < U<FULL>; ++k) {
-        const At<FULL> a(at, k, J.n);
-        c[k] = load_codes(J.codes + a.i, a.left);
-        e[k] = J.exps[a.i / 128];
+        const At<FULL> a(at, k, n);
+        c[k] = load_codes(codes + a.i, a.left);
+        e[k] = exps[a.i / 128];
     }
 #pragma unroll
-    for (int k = 0; k < U<FULL>; ++k) At<FULL>(at, k, J.n).store(J.out, decode4<SIGNED>(c[k], e[k]));
+    for (int k = 0; k < U<FULL>; ++k) At<FULL>(at, k, n).store(out, decode4<SIGNED>(c[k], e[k]));
 }
 template <bool SIGNED>
 __global__ __launch_bounds__(256) void k_moment_values(UJobs P) {
-    const int j = find_job(P);
-    const UJob& J = P.j[j];
-    const unsigned at = (blockIdx.x - J.first) * CHUNK;
-    if (at + CHUNK <= J.n) values_chunk<SIGNED, true>(J, at);
-    else each_part(at, J.n, [&](unsigned i) { values_chunk<SIGNED, false>(J, i); });
+    const int j = P.mine();
+    const unsigned at = (blockIdx.x - P.where(j).first) * CHUNK, n = P.j[j].n;
+    const uint8_t *codes = P.at<const uint8_t>(j, 0), *exps = P.at<const uint8_t>(j, 1);
+    float* out = P.at<float>(j, 2);
+    if (at + CHUNK <= n) values_chunk<SIGNED, true>(codes, exps, out, n, at);
+    else each_part(at, n, [&](unsigned i) { values_chunk<SIGNED, false>(codes, exps, out, n, i); });
 }
 
 // ------------------------------------------------------------------------------------------------------------- host
@@ -537,14 +561,14 @@ struct Ranges {
     }
 };
 
-// Splits a list into launches: `put(job, offset, count)` fills one job, `go(jobs, workgroups)` launches what has gathered.
-template <typename JOBS, typename PUT, typename GO>
-int each_launch(JOBS& P, const ayolo_tensor* t, int n, PUT put, GO go) {
+// Splits a list into launches.  where(i, off, address): a job's addresses, from element `off` of tensor i on; tag(i, part): its two
+// bits; go(jobs, workgroups) launches what has gathered.
+template <typename JOBS, typename WHERE, typename TAG, typename GO>
+int each_launch(JOBS& P, const ayolo_tensor* t, int n, const int (&unit)[JOBS::ADDRESSES], WHERE where, TAG tag, GO go) {
     unsigned wgs = 0;
     P.njobs = 0;
     auto flush = [&]() -> int {
-        if (P.njobs == 0) return AYOLO_OK;
-        const int rc = go(P, wgs);
+        const int rc = P.njobs ? go(P, wgs) : AYOLO_OK;
         P.njobs = 0;
         wgs = 0;
         return rc;
@@ -552,18 +576,23 @@ int each_launch(JOBS& P, const ayolo_tensor* t, int n, PUT put, GO go) {
     for (int i = 0; i < n; ++i) {
         if (!t[i].present) continue;
         for (int64_t off = 0; off < t[i].numel; off += PART) {
-            const unsigned cnt = (unsigned)std::min<int64_t>(PART, t[i].numel - off);
-            if (P.njobs == JOBS::MAX || wgs >= MOST_WGS) {
-                if (const int rc = flush()) return rc;
+            char* a[JOBS::ADDRESSES];
+            where(i, off, a);
+            bool fits = P.njobs > 0 && P.njobs < JOBS::MAX && wgs < MOST_WGS && (unsigned)i - P.tensor0 < 512u;
+            for (int k = 0; k < JOBS::ADDRESSES && fits; ++k) {
+                const int64_t d = (int64_t)((uintptr_t)a[k] - (uintptr_t)P.base[k]) / unit[k];
+                fits = d >= INT32_MIN && d <= INT32_MAX;
             }
-            auto& J = P.j[P.njobs];
-            if (const int rc = put(J, i, off, flush)) return rc;
-            auto& K = P.j[P.njobs];                        // `put` may have flushed
-            K = J;
-            K.n = cnt;
-            K.first = wgs;
-            wgs += (cnt + CHUNK - 1) / CHUNK;
-            ++P.njobs;
+            if (!fits) {
+                if (const int rc = flush()) return rc;
+                for (int k = 0; k < JOBS::ADDRESSES; ++k) P.base[k] = a[k];
+                P.tensor0 = (unsigned)i;
+            }
+            auto& J = P.j[P.njobs++];
+            for (int k = 0; k < JOBS::ADDRESSES; ++k) J.off[k] = (int)((int64_t)((uintptr_t)a[k] - (uintptr_t)P.base[k]) / unit[k]);
+            J.n = (unsigned)std::min<int64_t>(PART, t[i].numel - off);
+            J.meta = wgs | tag(i, (unsigned)(off / PART)) << 21 | ((unsigned)i - P.tensor0) << 23;
+            wgs += (J.n + CHUNK - 1) / CHUNK;
         }
     }
     return flush();
@@ -575,6 +604,12 @@ int64_t chunks_of(const ayolo_tensor* t, int n) {
         if (t[i].present)
             for (int64_t off = 0; off < t[i].numel; off += PART) c += cdiv64(std::min<int64_t>(PART, t[i].numel - off), CHUNK);
     return c;
+}
+
+template <typename GO>
+int grad_launches(GJobs& P, const ayolo_tensor* grads, int n, GO go) {
+    return each_launch(P, grads, n, {2}, [&](int i, int64_t off, char** a) { a[0] = (char*)grads[i].data + off * es_of(grads[i].dtype); },
+                       [&](int i, unsigned) { return (unsigned)grads[i].dtype; }, go);
 }
 
 }  // namespace
@@ -591,15 +626,13 @@ extern "C" int ayolo_grad_norm(const ayolo_tensor* grads, int n, const float* gr
     if (!ws || ws_bytes < ayolo_grad_norm_workspace(grads, n)) { ayolo_set_error("grad_norm: workspace %zu < %zu", ws_bytes, ayolo_grad_norm_workspace(grads, n)); return AYOLO_ENOSPC; }
     hipStream_t s = (hipStream_t)st;
     GJobs P{};
-    P.part = (double*)ws;
-    const int rc = each_launch(P, grads, n,
-        [&](GJob& J, int i, int64_t off, auto&&) { J.g = (char*)grads[i].data + off * es_of(grads[i].dtype); J.dtype = grads[i].dtype; return AYOLO_OK; },
-        [&](GJobs& Q, unsigned wgs) {
-            hipLaunchKernelGGL(k_grad_squares, dim3(wgs), dim3(256), 0, s, Q);
-            Q.part += wgs;
-            AY_CHECK_LAUNCH("k_grad_squares");
-            return AYOLO_OK;
-        });
+    P.h.part = (double*)ws;
+    const int rc = grad_launches(P, grads, n, [&](GJobs& Q, unsigned wgs) {
+        hipLaunchKernelGGL(k_grad_squares, dim3(wgs), dim3(256), 0, s, Q);
+        Q.h.part += wgs;
+        AY_CHECK_LAUNCH("k_grad_squares");
+        return AYOLO_OK;
+    });
     if (rc) return rc;
     hipLaunchKernelGGL(k_grad_norm, dim3(1), dim3(1024), 0, s, (const double*)ws, chunks, grad_scale, norm);
     AY_CHECK_LAUNCH("k_grad_norm");
@@ -617,15 +650,13 @@ extern "C" int ayolo_grad_clip(const ayolo_tensor* grads, int n, const float* no
     } catch (...) { ayolo_set_error("grad_clip: out of host memory"); return AYOLO_ENOSPC; }
     hipStream_t s = (hipStream_t)st;
     GJobs P{};
-    P.norm = norm;
-    P.max_norm = max_norm;
-    return each_launch(P, grads, n,
-        [&](GJob& J, int i, int64_t off, auto&&) { J.g = (char*)grads[i].data + off * es_of(grads[i].dtype); J.dtype = grads[i].dtype; return AYOLO_OK; },
-        [&](GJobs& Q, unsigned wgs) {
-            hipLaunchKernelGGL(k_grad_clip, dim3(wgs), dim3(256), 0, s, Q);
-            AY_CHECK_LAUNCH("k_grad_clip");
-            return AYOLO_OK;
-        });
+    P.h.norm = norm;
+    P.h.max_norm = max_norm;
+    return grad_launches(P, grads, n, [&](GJobs& Q, unsigned wgs) {
+        hipLaunchKernelGGL(k_grad_clip, dim3(wgs), dim3(256), 0, s, Q);
+        AY_CHECK_LAUNCH("k_grad_clip");
+        return AYOLO_OK;
+    });
 }
 
 namespace {
@@ -633,7 +664,7 @@ template <bool BITS8>
 int adamw_launches(const ayolo_adamw_list& L, const Hyper& h, hipStream_t s) {
     AJobs<BITS8> P{};
     P.h = h;
-    int dtype = -1;                                        // of the jobs that have gathered
+    int dtype = -1;                                        // of the jobs that have gathered: a launch has one
     auto go = [&](AJobs<BITS8>& Q, unsigned wgs) {
         if (dtype == AYOLO_F32) hipLaunchKernelGGL((k_adamw<float, BITS8>), dim3(wgs), dim3(256), 0, s, Q);
         else if (dtype == AYOLO_F16) hipLaunchKernelGGL((k_adamw<half_t, BITS8>), dim3(wgs), dim3(256), 0, s, Q);
@@ -641,28 +672,36 @@ int adamw_launches(const ayolo_adamw_list& L, const Hyper& h, hipStream_t s) {
         AY_CHECK_LAUNCH("k_adamw");
         return AYOLO_OK;
     };
-    auto put = [&](AJob<BITS8>& J, int i, int64_t off, auto&& flush) {
-        if (L.p[i].dtype != dtype) {
-            if (const int rc = flush()) return rc;
-            dtype = L.p[i].dtype;
+    int from = 0;
+    while (from < L.n) {                                   // runs of one type
+        int to = from;
+        dtype = -1;
+        for (; to < L.n; ++to) {
+            if (!L.g[to].present) continue;
+            if (dtype >= 0 && L.p[to].dtype != dtype) break;
+            dtype = L.p[to].dtype;
         }
         const int es = es_of(dtype);
-        J.p = (char*)L.p[i].data + off * es;
-        J.g = (const char*)L.g[i].data + off * es;
-        if constexpr (BITS8) {
-            J.m = (uint8_t*)L.m[i].data + off;
-            J.v = (uint8_t*)L.v[i].data + off;
-            J.me = (uint8_t*)L.me[i].data + off / 128;
-            J.ve = (uint8_t*)L.ve[i].data + off / 128;
-        } else {
-            J.m = (float*)L.m[i].data + off;
-            J.v = (float*)L.v[i].data + off;
-        }
-        J.tensor = (unsigned)i;
-        J.origin = (unsigned)off;
-        return AYOLO_OK;
-    };
-    return each_launch(P, L.g, L.n, put, go);
+        auto where = [&](int i, int64_t off, char** a) {
+            i += from;
+            a[0] = (char*)L.p[i].data + off * es;
+            a[1] = (char*)L.g[i].data + off * es;
+            a[2] = (char*)L.m[i].data + off * (BITS8 ? 1 : 4);
+            a[3] = (char*)L.v[i].data + off * (BITS8 ? 1 : 4);
+            if constexpr (BITS8) {
+                a[4] = (char*)L.me[i].data + off / 128;
+                a[5] = (char*)L.ve[i].data + off / 128;
+            }
+        };
+        auto part = [](int, unsigned p) { return p & 3u; };
+        P.h.coef = h.coef + from;
+        int rc;
+        if constexpr (BITS8) rc = each_launch(P, L.g + from, to - from, {es, es, 1, 1, 1, 1}, where, part, go);
+        else rc = each_launch(P, L.g + from, to - from, {es, es, 4, 4}, where, part, go);
+        if (rc) return rc;
+        from = to;
+    }
+    return AYOLO_OK;
 }
 }  // namespace
 
@@ -727,21 +766,36 @@ extern "C" int ayolo_adamw_step(const ayolo_adamw_list* L, const ayolo_adamw_hyp
     Q.found_inf = H->found_inf;
     Q.out = (Coef*)ws;
     Q.seed = H->seed;
-    for (int base = 0; base < n; base += PrepJobs::MAX) {
-        Q.base = base;
-        Q.n = std::min(n - base, (int)PrepJobs::MAX);
-        bool any = false;
-        for (int i = 0; i < Q.n; ++i) {
-            const bool on = L->g[base + i].present;
-            any |= on;
-            Q.j[i].step = on ? (float*)L->step[base + i].data : nullptr;
-            Q.j[i].lr = L->lr ? L->lr[base + i] : H->lr;
-            Q.j[i].wd = L->weight_decay ? L->weight_decay[base + i] : H->weight_decay;
-        }
-        if (!any) continue;
-        hipLaunchKernelGGL(k_adamw_prepare, dim3(1), dim3(256), 0, s, Q);
+    auto prepare = [&]() -> int {
+        if (Q.n == 0) return AYOLO_OK;
+        hipLaunchKernelGGL(k_adamw_prepare, dim3(1), dim3(512), 0, s, Q);
         AY_CHECK_LAUNCH("k_adamw_prepare");
+        Q.n = 0;
+        return AYOLO_OK;
+    };
+    for (int i = 0; i < n; ++i) {
+        if (!L->g[i].present) continue;
+        const float lr = L->lr ? L->lr[i] : H->lr, wd = L->weight_decay ? L->weight_decay[i] : H->weight_decay;
+        int pair = 0;
+        if (Q.n)
+            while (pair < Q.pairs && !(Q.pair[pair].lr == lr && Q.pair[pair].wd == wd)) ++pair;
+        const int64_t d = Q.n ? (int64_t)((uintptr_t)L->step[i].data - (uintptr_t)Q.step) / 4 : 0;
+        if (Q.n == 0 || Q.n == PrepJobs::MAX || pair == PrepJobs::PAIRS || d < INT32_MIN || d > INT32_MAX || (unsigned)i - Q.place0 >= 1u << 26) {
+            if (const int rc = prepare()) return rc;
+            Q.step = (char*)L->step[i].data;
+            Q.place0 = (unsigned)i;
+            Q.pairs = pair = 0;
+        }
+        if (pair == Q.pairs) {
+            Q.pair[pair].lr = lr;
+            Q.pair[pair].wd = wd;
+            ++Q.pairs;
+        }
+        Q.j[Q.n].off = (int)((int64_t)((uintptr_t)L->step[i].data - (uintptr_t)Q.step) / 4);
+        Q.j[Q.n].which = (unsigned)pair | ((unsigned)i - Q.place0) << 6;
+        ++Q.n;
     }
+    if (const int rc = prepare()) return rc;
     Hyper h{};
     h.grad_scale = H->grad_scale;
     h.found_inf = H->found_inf;
@@ -770,13 +824,13 @@ extern "C" int ayolo_moment_values(const ayolo_tensor* codes, const ayolo_tensor
     }
     hipStream_t s = (hipStream_t)st;
     UJobs P{};
-    return each_launch(P, codes, n,
-        [&](UJob& J, int i, int64_t off, auto&&) {
-            J.codes = (const uint8_t*)codes[i].data + off;
-            J.exps = (const uint8_t*)exps[i].data + off / 128;
-            J.out = (float*)out[i].data + off;
-            return AYOLO_OK;
+    return each_launch(P, codes, n, {1, 1, 4},
+        [&](int i, int64_t off, char** a) {
+            a[0] = (char*)codes[i].data + off;
+            a[1] = (char*)exps[i].data + off / 128;
+            a[2] = (char*)out[i].data + off * 4;
         },
+        [](int, unsigned) { return 0u; },
         [&](UJobs& Q, unsigned wgs) {
             if (is_signed) hipLaunchKernelGGL(k_moment_values<true>, dim3(wgs), dim3(256), 0, s, Q);
             else hipLaunchKernelGGL(k_moment_values<false>, dim3(wgs), dim3(256), 0, s, Q);
