@@ -218,11 +218,12 @@ def call(name: str, *args) -> None:
 def call_on(device: int, name: str, *args) -> None:
     """call() with the current stream of device `device` as the last argument, that device being current."""
     import torch
-    if torch.cuda.current_device() == device:
-        check(getattr(lib(), name)(*args, torch.cuda.current_stream().cuda_stream), name)
+    fn, stream = getattr(lib(), name), torch._C._cuda_getCurrentRawStream(device)
+    if torch._C._cuda_getDevice() == device:
+        check(fn(*args, stream), name)
         return
     with torch.cuda.device(device):
-        check(getattr(lib(), name)(*args, torch.cuda.current_stream().cuda_stream), name)
+        check(fn(*args, stream), name)
 
 
 _host = None

@@ -183,16 +183,22 @@ def grad_norm(grads: Sequence[Optional[torch.Tensor]], grad_scale: Optional[torc
     dev = _device_of(grads, "grad_norm")
     if dev is None:
         return torch.zeros(())
-    rows = _lib.tensor_rows(grads, "grad_norm")
-    info = np.frombuffer(rows, dtype=_TENSOR)
-    if ((info["layout"] == 0) & (info["present"] != 0)).any():       # an expanded or strided gradient: its elements in a block
-        grads = [g if g is None else g.contiguous() for g in grads]
-        rows = _lib.tensor_rows(grads, "grad_norm")
+    return _norm(grads, _lib.tensor_rows(grads, "grad_norm"), dev, grad_scale)
+
+
+def _norm(grads, rows: bytes, dev: torch.device, grad_scale: Optional[torch.Tensor] = None) -> torch.Tensor:
+    scale = _scalar(grad_scale, dev, "grad_norm", "grad_scale")
     need = int(_lib.lib().ayolo_grad_norm_workspace(rows, len(grads)))
-    ws = torch.empty(need, dtype=torch.uint8, device=dev)
-    norm = torch.empty((), dtype=torch.float32, device=dev)
-    _lib.call_on(dev.index, "ayolo_grad_norm", rows, len(grads), _scalar(grad_scale, dev, "grad_norm", "grad_scale"), norm.data_ptr(),
-                 ws.data_ptr(), need)
+    ws, norm = torch.empty(need, dtype=torch.uint8, device=dev), torch.empty((), dtype=torch.float32, device=dev)
+    try:
+        _lib.call_on(dev.index, "ayolo_grad_norm", rows, len(grads), scale, norm.data_ptr(), ws.data_ptr(), need)
+    except _lib.AyoloError:
+        info = np.frombuffer(rows, dtype=_TENSOR)
+        if not ((info["layout"] == 0) & (info["present"] != 0)).any():
+            raise
+        # an expanded or strided gradient (the call launches nothing then): the norm of its elements in a block
+        grads = [g if g is None else g.contiguous() for g in grads]
+        return _norm(grads, _lib.tensor_rows(grads, "grad_norm"), dev, grad_scale)
     return norm
 
 
@@ -207,10 +213,10 @@ def clip_grads_(grads: Sequence[Optional[torch.Tensor]], max_norm: float, norm: 
     dev = _device_of(grads, "clip_grads_")
     if dev is None:
         return torch.zeros(()) if norm is None else norm
+    rows = _lib.tensor_rows(grads, "clip_grads_")
     if norm is None:
-        norm = grad_norm(grads)
-    _lib.call_on(dev.index, "ayolo_grad_clip", _lib.tensor_rows(grads, "clip_grads_"), len(grads), _scalar(norm, dev, "clip_grads_", "norm"),
-                 max_norm)
+        norm = _norm(grads, rows, dev)
+    _lib.call_on(dev.index, "ayolo_grad_clip", rows, len(grads), _scalar(norm, dev, "clip_grads_", "norm"), max_norm)
     _lib.host().bump(grads, grads)
     return norm
 
@@ -299,15 +305,7 @@ def adamw_step(params: Sequence[torch.Tensor], grads: Sequence[Optional[torch.Te
     bits8 = isinstance(next((m for m in exp_avgs if m is not None), None), (tuple, list))      # pairs throughout, or tensors
     rows = _lib.tensor_rows
     L, H = _lib.AdamWList(), _lib.AdamWHyper()
-    prows, grows = rows(params, "adamw_step: params"), rows(grads, "adamw_step: grads")
-    pi, gi = np.frombuffer(prows, dtype=_TENSOR), np.frombuffer(grows, dtype=_TENSOR)
-    other = (gi["present"] != 0) & (pi["layout"] != gi["layout"])
-    if other.any():                                # a gradient in another memory order than its parameter: laid out like it
-        for i in np.flatnonzero(other):
-            if torch.is_tensor(params[i]) and params[i].shape == grads[i].shape:
-                grads[i] = SGD._dense_like(params[i], grads[i])
-        grows = rows(grads, "adamw_step: grads")
-    L.n, L.p, L.g = n, prows, grows
+    L.n, L.p, L.g = n, rows(params, "adamw_step: params"), rows(grads, "adamw_step: grads")
     if bits8:
         L.m, L.me = rows(exp_avgs, "adamw_step: exp_avgs", 0), rows(exp_avgs, "adamw_step: exp_avgs", 1)
         L.v, L.ve = rows(exp_avg_sqs, "adamw_step: exp_avg_sqs", 0), rows(exp_avg_sqs, "adamw_step: exp_avg_sqs", 1)
@@ -327,7 +325,19 @@ def adamw_step(params: Sequence[torch.Tensor], grads: Sequence[Optional[torch.Te
     H.maximize, H.seed = int(bool(maximize)), int(seed) & 0xFFFFFFFF
     need = int(_lib.lib().ayolo_adamw_workspace(n))
     ws = torch.empty(need, dtype=torch.uint8, device=dev)
-    _lib.call_on(dev.index, "ayolo_adamw_step", L, H, ws.data_ptr(), need)
+    try:
+        _lib.call_on(dev.index, "ayolo_adamw_step", L, H, ws.data_ptr(), need)
+    except _lib.AyoloError:
+        # a gradient in another memory order than its parameter (the call launches nothing then): laid out like it
+        pi, gi = (np.frombuffer(rows(t, "adamw_step"), dtype=_TENSOR) for t in (params, grads))
+        other = [i for i in np.flatnonzero((gi["present"] != 0) & (pi["layout"] != gi["layout"]) & (pi["layout"] != 0))
+                 if params[i].shape == grads[i].shape]
+        if not other:
+            raise
+        for i in other:
+            grads[i] = SGD._dense_like(params[i], grads[i])
+        L.g = rows(grads, "adamw_step: grads")
+        _lib.call_on(dev.index, "ayolo_adamw_step", L, H, ws.data_ptr(), need)
     _lib.host().bump(params, grads)                # written through raw pointers
 
 
