@@ -3,8 +3,10 @@
 // norm's checks, buffers and autograd node (a norm of a few rows takes the GPU 3 us, a node written in Python 25 us of host time
 // forward and, in autograd's own thread, 40 us backward).  No arithmetic here: the kernels are reached through the C ABI, whose
 // addresses bind() is given.
-#include <torch/csrc/autograd/custom_function.h>
+#include <torch/csrc/autograd/function.h>
 #include <torch/csrc/autograd/functions/basic_ops.h>
+#include <torch/csrc/autograd/functions/utils.h>
+#include <torch/csrc/autograd/saved_variable.h>
 #include <torch/csrc/Exceptions.h>
 #include <torch/csrc/autograd/python_variable.h>
 
@@ -20,7 +22,6 @@
 namespace {
 
 using at::Tensor;
-using torch::autograd::AutogradContext;
 using torch::autograd::variable_list;
 
 PyObject* ayolo_error = nullptr;      // _lib.AyoloError
@@ -165,113 +166,134 @@ void checked(int rc, const char* what) {
 at::ScalarType params_type(const Tensor& w, const Tensor& b, at::ScalarType dt) {
     return (w.defined() || b.defined()) && (!w.defined() || w.scalar_type() == dt) && (!b.defined() || b.scalar_type() == dt) ? dt : at::kFloat;
 }
-Tensor as_param(const Tensor& t, at::ScalarType dt) { return t.defined() ? t.detach().to(dt).contiguous() : t; }
+Tensor as_param(const Tensor& t, at::ScalarType dt) { return t.defined() ? t.to(dt).contiguous() : t; }      // t itself where it fits
 
+// x laid out so that dimension `dim` is innermost
+Tensor empty_along(const Tensor& x, int64_t dim) {
+    at::DimVector strides(x.dim());
+    int64_t n = 1;
+    strides[dim] = 1;
+    n *= x.size(dim);
+    for (int64_t d = x.dim() - 1; d >= 0; --d) {
+        if (d == dim) continue;
+        strides[d] = n;
+        n *= std::max<int64_t>(x.size(d), 1);
+    }
+    return at::empty_strided(x.sizes(), strides, x.options());
+}
+Tensor along(const Tensor& t, int64_t dim) { return !t.defined() || dim == t.dim() - 1 ? t : t.movedim(dim, -1); }
+void* stream_of(const Tensor& t) { return c10::hip::getCurrentHIPStream(t.device().index()).stream(); }
+
+// Below autograd (no views or graph are recorded in here).
 struct Norm { Tensor y, s, mean, rstd, w; };
 Norm norm_forward(const Tensor& x0, const Tensor& r0, const Tensor& w0, const Tensor& b0, double eps, int64_t dim, bool stats) {
+    const at::AutoDispatchBelowADInplaceOrView below;
     const c10::DeviceGuard guard(x0.device());
     const at::ScalarType wdt = params_type(w0, b0, x0.scalar_type());
-    const bool last = dim == x0.dim() - 1;
-    Tensor x = last ? x0 : x0.movedim(dim, -1), r = !r0.defined() || last ? r0 : r0.movedim(dim, -1);
+    Tensor x = along(x0, dim), r = along(r0, dim);
     const int64_t C = x.size(-1), n = x.numel() / C;
     Norm o;
     o.w = as_param(w0, wdt);
     const Tensor b = as_param(b0, wdt);
-    o.y = at::empty(x.sizes(), x.options());
-    if (r.defined()) o.s = at::empty(x.sizes(), x.options());
+    o.y = empty_along(x0, dim);
+    if (r.defined()) o.s = empty_along(x0, dim);
     if (stats) {
-        const Tensor both = at::empty({2, n}, x.options().dtype(at::kFloat));
-        o.mean = both.select(0, 0);
-        o.rstd = both.select(0, 1);
+        o.mean = at::empty({n}, x.options().dtype(at::kFloat));
+        o.rstd = at::empty({n}, x.options().dtype(at::kFloat));
     }
     const int dt = dtype_of(x);
     const ayolo_rows xr = row_view(x);
     ayolo_rows rr{};
     if (r.defined()) rr = row_view(r);
     checked(f_fwd(dt, &xr, r.defined() ? &rr : nullptr, n, C, ptr(o.w), ptr(b), wdt == at::kFloat ? AYOLO_F32 : dt, (float)eps, ptr(o.y),
-                  ptr(o.s), (float*)ptr(o.mean), (float*)ptr(o.rstd), c10::hip::getCurrentHIPStream(x.device().index()).stream()),
+                  ptr(o.s), (float*)ptr(o.mean), (float*)ptr(o.rstd), stream_of(x)),
             "ayolo_layer_norm_fwd");
-    if (!last) {
-        o.y = o.y.movedim(-1, dim);
-        if (o.s.defined()) o.s = o.s.movedim(-1, dim);
-    }
     return o;
 }
 
-struct LayerNorm : torch::autograd::Function<LayerNorm> {
-    static variable_list forward(AutogradContext* ctx, const Tensor& x, const std::optional<Tensor>& residual, const std::optional<Tensor>& weight,
-                                 const std::optional<Tensor>& bias, double eps, int64_t dim) {
-        const Tensor r = residual.value_or(Tensor()), w = weight.value_or(Tensor()), b = bias.value_or(Tensor());
-        const Norm o = norm_forward(x, r, w, b, eps, dim, true);
-        ctx->set_materialize_grads(false);
-        ctx->save_for_backward({r.defined() ? o.s : x, o.w, o.mean, o.rstd});
-        auto& kept = ctx->saved_data;
-        kept["dim"] = dim;
-        kept["wtype"] = w.defined() ? (int64_t)w.scalar_type() : -1;
-        kept["btype"] = b.defined() ? (int64_t)b.scalar_type() : -1;
-        kept["ptype"] = (int64_t)params_type(w, b, x.scalar_type());
-        kept["need_x"] = x.requires_grad();
-        kept["need_r"] = r.defined() && r.requires_grad();
-        kept["need_w"] = w.defined() && w.requires_grad();
-        kept["need_b"] = b.defined() && b.requires_grad();
-        if (r.defined()) return {o.y, o.s};
-        return {o.y};
+// Its edges: x, residual, weight, bias.
+struct LayerNormBackward : torch::autograd::Node {
+    torch::autograd::SavedVariable s, w, mean, rstd;
+    int64_t dim = 0;
+    bool sum_kept = false;                                 // s is this node's output (the residual sum), not its input
+    at::ScalarType ptype = at::kFloat, wtype = at::kFloat, btype = at::kFloat;
+
+    std::string name() const override { return "LayerNormBackward"; }
+    void release_variables() override {
+        const std::lock_guard<std::mutex> lock(mutex_);
+        s.reset_data();
+        w.reset_data();
+        mean.reset_data();
+        rstd.reset_data();
     }
 
-    static variable_list backward(AutogradContext* ctx, const variable_list& grads) {
-        const variable_list saved = ctx->get_saved_variables();
-        auto& kept = ctx->saved_data;
-        const int64_t dim = kept["dim"].toInt();
-        const bool nx = kept["need_x"].toBool(), nr = kept["need_r"].toBool(), nw = kept["need_w"].toBool(), nb = kept["need_b"].toBool();
-        Tensor s = saved[0], dy = grads[0], q = grads.size() > 1 ? grads[1] : Tensor();
-        Tensor dx, dw, db;
+    variable_list apply(variable_list&& grads) override {
+        const std::lock_guard<std::mutex> lock(mutex_);
+        const bool nx = task_should_compute_output(0), nr = task_should_compute_output(1), nw = task_should_compute_output(2),
+                   nb = task_should_compute_output(3);
+        Tensor dy = grads[0], q = grads.size() > 1 ? grads[1] : Tensor(), dx, dw, db;
+        variable_list out(4);
         if (!dy.defined()) {                               // only the residual sum was used
-            dx = q;
-        } else {
-            const at::NoGradGuard no_grad;
-            const c10::DeviceGuard guard(s.device());
-            const bool last = dim == s.dim() - 1;
-            const at::ScalarType wdt = (at::ScalarType)kept["ptype"].toInt();
-            dy = dy.to(s.scalar_type());
-            if (q.defined()) q = q.to(s.scalar_type());
-            if (!last) {
-                s = s.movedim(dim, -1);
-                dy = dy.movedim(dim, -1);
-                if (q.defined()) q = q.movedim(dim, -1);
-            }
-            const int64_t C = s.size(-1), n = s.numel() / C;
-            const int dt = dtype_of(s);
-            if (nx || nr) dx = at::empty(s.sizes(), s.options());
-            if (nw) dw = at::empty({C}, s.options().dtype(wdt));
-            if (nb) db = at::empty({C}, s.options().dtype(wdt));
+            out[0] = nx ? q : Tensor();
+            out[1] = nr ? q : Tensor();
+            return out;
+        }
+        {
+            const Tensor s0 = s.unpack(sum_kept ? shared_from_this() : nullptr), gain = w.unpack(), mu = mean.unpack(), rs = rstd.unpack();
+            const at::AutoDispatchBelowADInplaceOrView below;
+            const c10::DeviceGuard guard(s0.device());
+            Tensor x = along(s0, dim);
+            dy = along(dy.scalar_type() == x.scalar_type() ? dy : dy.to(x.scalar_type()), dim);
+            if (q.defined()) q = along(q.scalar_type() == x.scalar_type() ? q : q.to(x.scalar_type()), dim);
+            const int64_t C = x.size(-1), n = x.numel() / C;
+            const int dt = dtype_of(x);
+            if (nx || nr) dx = empty_along(s0, dim);
+            if (nw) dw = at::empty({C}, x.options().dtype(ptype));
+            if (nb) db = at::empty({C}, x.options().dtype(ptype));
             const size_t need = nw || nb ? f_ws(dt, n, C) : 0;
-            const Tensor ws = need ? at::empty({(int64_t)need}, s.options().dtype(at::kByte)) : Tensor();
-            const ayolo_rows sr = row_view(s), gr = row_view(dy);
+            const Tensor ws = need ? at::empty({(int64_t)need}, x.options().dtype(at::kByte)) : Tensor();
+            const ayolo_rows sr = row_view(x), gr = row_view(dy);
             ayolo_rows qr{};
             if (q.defined()) qr = row_view(q);
-            checked(f_bwd(dt, &sr, &gr, q.defined() ? &qr : nullptr, n, C, ptr(saved[1]), wdt == at::kFloat ? AYOLO_F32 : dt,
-                          (const float*)ptr(saved[2]), (const float*)ptr(saved[3]), ptr(dx), ptr(dw), ptr(db), ptr(ws), need,
-                          c10::hip::getCurrentHIPStream(s.device().index()).stream()),
+            checked(f_bwd(dt, &sr, &gr, q.defined() ? &qr : nullptr, n, C, ptr(gain), ptype == at::kFloat ? AYOLO_F32 : dt, (const float*)ptr(mu),
+                          (const float*)ptr(rs), ptr(dx), ptr(dw), ptr(db), ptr(ws), need, stream_of(x)),
                     "ayolo_layer_norm_bwd");
-            if (!last && dx.defined()) dx = dx.movedim(-1, dim);
-            if (nw) dw = dw.to((at::ScalarType)kept["wtype"].toInt());
-            if (nb) db = db.to((at::ScalarType)kept["btype"].toInt());
+            if (nw && wtype != ptype) dw = dw.to(wtype);
+            if (nb && btype != ptype) db = db.to(btype);
         }
-        variable_list out = {nx ? dx : Tensor(), nr ? dx : Tensor(), dw, db, Tensor(), Tensor()};
+        out = {nx ? dx : Tensor(), nr ? dx : Tensor(), dw, db};
         if (at::GradMode::is_enabled()) {                  // create_graph: what was computed here has no derivative
             variable_list given;
-            for (int k = 0; k < 4; ++k)
-                if (out[k].defined()) given.push_back(out[k].detach());
-            auto stop = std::make_shared<torch::autograd::DelayedError>("layer_norm is differentiable once", (int)given.size());
-            for (auto& t : given) t.requires_grad_(true);
-            variable_list marked = (*stop)(std::move(given));
+            for (auto& t : out)
+                if (t.defined()) given.push_back(t.detach().requires_grad_(true));
+            const auto stop = std::make_shared<torch::autograd::DelayedError>("layer_norm is differentiable once", (int)given.size());
+            const variable_list marked = (*stop)(std::move(given));
             size_t at = 0;
-            for (int k = 0; k < 4; ++k)
-                if (out[k].defined()) out[k] = marked[at++];
+            for (auto& t : out)
+                if (t.defined()) t = marked[at++];
         }
         return out;
     }
 };
+
+variable_list norm_with_graph(const Tensor& x, const Tensor& r, const Tensor& w, const Tensor& b, double eps, int64_t dim) {
+    Norm o = norm_forward(x, r, w, b, eps, dim, true);
+    const std::shared_ptr<LayerNormBackward> node(new LayerNormBackward(), torch::autograd::deleteNode);
+    node->set_next_edges(torch::autograd::collect_next_edges(x, r, w, b));
+    node->dim = dim;
+    node->sum_kept = r.defined();
+    node->ptype = params_type(w, b, x.scalar_type());
+    if (w.defined()) node->wtype = w.scalar_type();
+    if (b.defined()) node->btype = b.scalar_type();
+    variable_list out = {o.y};
+    if (r.defined()) out.push_back(o.s);
+    torch::autograd::set_history(out, node);
+    node->s = torch::autograd::SavedVariable(r.defined() ? out[1] : x, r.defined());
+    node->w = torch::autograd::SavedVariable(o.w, false);
+    node->mean = torch::autograd::SavedVariable(o.mean, false);
+    node->rstd = torch::autograd::SavedVariable(o.rstd, false);
+    return out;
+}
 
 // layer_norm(x, weight, bias, eps, residual, dim): y, or (y, x + residual)
 PyObject* layer_norm(PyObject*, PyObject* args) {
@@ -301,13 +323,12 @@ PyObject* layer_norm(PyObject*, PyObject* args) {
         REFUSE_UNLESS(!r.defined() || (r.sizes() == x.sizes() && r.scalar_type() == x.scalar_type() && r.device() == x.device() && r.layout() == at::kStrided),
                       "layer_norm: residual must have x's shape ", x.sizes(), ", type ", x.scalar_type(), " and device ", x.device());
         REFUSE_UNLESS(eps >= 0.0, "layer_norm: eps=", eps);
+        for (const Tensor* t : {&x, &w, &b, &r}) REFUSE_UNLESS(!torch::autograd::isFwGradDefined(*t), "layer_norm has no forward-mode derivative");
         variable_list out;
         auto grad = [](const Tensor& t) { return t.defined() && t.requires_grad(); };
         if (at::GradMode::is_enabled() && (grad(x) || grad(r) || grad(w) || grad(b))) {
-            auto opt = [](const Tensor& t) { return t.defined() ? std::optional<Tensor>(t) : std::nullopt; };
-            out = LayerNorm::apply(x, opt(r), opt(w), opt(b), eps, (int64_t)dim);
+            out = norm_with_graph(x, r, w, b, eps, dim);
         } else {
-            const at::NoGradGuard no_grad;
             const Norm o = norm_forward(x, r, w, b, eps, dim, false);
             out.push_back(o.y);
             if (r.defined()) out.push_back(o.s);

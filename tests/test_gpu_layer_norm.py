@@ -214,6 +214,46 @@ def test_only_one_output_used():
     assert float((gx.double().cpu() - want).abs().max()) <= 64 * U * 64
 
 
+def test_differentiable_once():
+    """create_graph works as far as nobody asks for the derivative of a gradient; forward mode is refused; a weight changed in place
+    between forward and backward is noticed"""
+    from ayolov2_amd._lib import AyoloError
+    from ayolov2_amd.functional import layer_norm
+    x = _make((5, 24), torch.float32, 1).cuda().requires_grad_()
+    w = torch.ones(24, device="cuda", requires_grad=True)
+    y, s = layer_norm(x, w, residual=x.detach())
+    plain = torch.autograd.grad((y.sin().sum(), s.sum()), (x, w), retain_graph=True)
+    kept = torch.autograd.grad((y.sin().sum(), s.sum()), (x, w), create_graph=True)
+    for a, c in zip(plain, kept):
+        assert torch.equal(a, c)
+    with pytest.raises(RuntimeError, match="differentiable once"):
+        kept[0].sum().backward()
+    with torch.autograd.forward_ad.dual_level():
+        with pytest.raises(AyoloError, match="forward-mode"):
+            layer_norm(torch.autograd.forward_ad.make_dual(x.detach(), torch.ones_like(x)))
+    y = layer_norm(x, w)
+    with torch.no_grad():
+        w.mul_(2.0)
+    with pytest.raises(RuntimeError, match="modified by an inplace operation"):
+        y.sum().backward()
+
+
+def test_in_place_use_of_the_outputs():
+    """y may be changed in place (backward does not read it), the sum may not"""
+    from ayolov2_amd.functional import layer_norm
+    x = _make((2, 24, 3, 5), torch.float32, 1).cuda().requires_grad_()
+    gy = _make((2, 24, 3, 5), torch.float32, 2).cuda()
+    y = layer_norm(x, dim=1)
+    want = torch.autograd.grad(y, x, 2 * gy)[0]
+    y = layer_norm(x, dim=1)
+    y.mul_(2.0)
+    assert torch.equal(torch.autograd.grad(y, x, gy)[0], want)
+    y, s = layer_norm(x, residual=x.detach(), dim=1)
+    s.add_(1.0)
+    with pytest.raises(RuntimeError, match="modified by an inplace operation"):
+        (y + s).sum().backward()
+
+
 def test_gradient_against_differences():
     """Directional derivative of sum(y * g) by central differences of the kernel's own fp32 forward: step h = 2^-6, error
     h^2 / 6 * |third derivative| (about 1e-4 of the value at unit scale) + 2 * 64 u * |y g| / h."""
