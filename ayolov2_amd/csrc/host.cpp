@@ -63,6 +63,10 @@ PyObject* rows(PyObject*, PyObject* args) {
     PyObject* list;
     int item = -1;
     if (!PyArg_ParseTuple(args, "O|i", &list, &item)) return nullptr;
+    if (item > 1) {
+        PyErr_SetString(PyExc_ValueError, "item: 0 or 1");
+        return nullptr;
+    }
     PyObject* seq = PySequence_Fast(list, "a sequence of tensors is needed");
     if (!seq) return nullptr;
     const Py_ssize_t n = PySequence_Fast_GET_SIZE(seq);
@@ -72,16 +76,16 @@ PyObject* rows(PyObject*, PyObject* args) {
         ayolo_tensor row{};
         row.device = -1;
         PyObject* e = PySequence_Fast_GET_ITEM(seq, i);
-        PyObject* held = nullptr;
         if (e != Py_None && item >= 0) {
-            held = PySequence_Check(e) && !THPVariable_Check(e) ? PySequence_GetItem(e, item) : nullptr;
-            if (!held) {
-                PyErr_Clear();
+            const bool tuple = PyTuple_Check(e);
+            if (!tuple && !PyList_Check(e)) e = nullptr;
+            else if ((tuple ? PyTuple_GET_SIZE(e) : PyList_GET_SIZE(e)) != 2) e = nullptr;
+            else e = tuple ? PyTuple_GET_ITEM(e, item) : PyList_GET_ITEM(e, item);
+            if (!e) {
                 PyErr_Format(PyExc_TypeError, "entry %zd is not a (codes, exponents) pair", i);
                 ok = false;
                 break;
             }
-            e = held;
         }
         if (e != Py_None) {
             if (!THPVariable_Check(e)) {
@@ -103,7 +107,6 @@ PyObject* rows(PyObject*, PyObject* args) {
                 }
             }
         }
-        Py_XDECREF(held);
         if (ok) reinterpret_cast<ayolo_tensor*>(PyBytes_AS_STRING(out))[i] = row;
     }
     Py_DECREF(seq);
