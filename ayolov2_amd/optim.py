@@ -369,7 +369,8 @@ class AdamW(torch.optim.AdamW):
         """States of parameters that have a gradient for the first time."""
         if torch.cuda.is_current_stream_capturing():
             raise _lib.AyoloError("ayolov2_amd.optim.AdamW: run one step before capturing: a replay would start from new states")
-        for (p, st), t in zip(todo, torch.zeros(len(todo), dtype=torch.float32, device=todo[0][0].device).unbind()):
+        for p, t in zip(todo, torch.zeros(len(todo), dtype=torch.float32, device=todo[0].device).unbind()):
+            st = self.state[p]
             st["step"] = t
             if self.state_bits == 8:
                 m, v = new_moment8(p), new_moment8(p)
@@ -378,20 +379,25 @@ class AdamW(torch.optim.AdamW):
                 st["exp_avg"] = torch.zeros_like(p, dtype=torch.float32, memory_format=torch.preserve_format)
                 st["exp_avg_sq"] = torch.zeros_like(p, dtype=torch.float32, memory_format=torch.preserve_format)
 
-    def _moments(self, st):
-        if not st:
-            return None, None, None
+    def _states(self, ps, grads):
+        """(exp_avgs, exp_avg_sqs, steps) of a group's parameters; None for those that never had a gradient."""
+        get = self.state.get
+        sts = [get(p) for p in ps]
+        todo = [p for p, g, st in zip(ps, grads, sts) if g is not None and not st]
+        if todo:
+            self._new_states(todo)
+            sts = [get(p) for p in ps]
+        none = dict.fromkeys(("exp_avg", "exp_avg_sq", "exp_avg_exps", "exp_avg_sq_exps", "step"))
+        sts = [st or none for st in sts]
         if self.state_bits == 8:
-            return Moment8(st["exp_avg"], st["exp_avg_exps"]), Moment8(st["exp_avg_sq"], st["exp_avg_sq_exps"]), st["step"]
-        return st["exp_avg"], st["exp_avg_sq"], st["step"]
+            pairs = (lambda name: [None if st is none else (st[name], st[name + "_exps"]) for st in sts])
+            return pairs("exp_avg"), pairs("exp_avg_sq"), [st["step"] for st in sts]
+        return [st["exp_avg"] for st in sts], [st["exp_avg_sq"] for st in sts], [st["step"] for st in sts]
 
     @torch.no_grad()
     def step(self, closure=None):
         scale, found = getattr(self, "grad_scale", None), getattr(self, "found_inf", None)
-        on_gpu = {p.is_cuda for g in self.param_groups for p in g["params"] if p.grad is not None}
-        if len(on_gpu) == 2:
-            raise _lib.AyoloError("ayolov2_amd.optim.AdamW: parameters on the CPU and on the GPU")
-        if on_gpu == {False}:
+        if not next((p.is_cuda for g in self.param_groups for p in g["params"]), True):
             if self.state_bits == 8 or scale is not None or found is not None:
                 raise _lib.AyoloError("ayolov2_amd.optim.AdamW: 8-bit states and the GradScaler hand-over need parameters on the GPU")
             if self.max_norm is not None:
@@ -403,39 +409,29 @@ class AdamW(torch.optim.AdamW):
         if closure is not None:
             with torch.enable_grad():
                 loss = closure()
-        runs, todo, grads = {}, [], []
+        runs = {}
         for k, g in enumerate(self.param_groups):
             if g.get("amsgrad"):
                 raise _lib.AyoloError("ayolov2_amd.optim.AdamW: amsgrad has no kernel")
-            lr = g["lr"]
+            lr, ps = g["lr"], g["params"]
             if torch.is_tensor(lr) and not lr.is_cuda:
                 lr = float(lr)
             # groups that differ in learning rate and decay alone share their launches
             key = (tuple(g["betas"]), g["eps"], bool(g["maximize"]), k if torch.is_tensor(lr) else -1)
-            run = runs.setdefault(key, ([], [], [], [], lr))
-            for p in g["params"]:
-                st = self.state[p] if p.grad is not None else self.state.get(p, {})
-                if p.grad is not None:
-                    if p.grad.is_sparse:
-                        raise _lib.AyoloError("ayolov2_amd.optim.AdamW: sparse gradients have no kernel")
-                    if not st:
-                        todo.append((p, st))
-                    grads.append(p.grad)
-                run[0].append(p)
-                run[1].append(st)
-                run[2].append(lr)
-                run[3].append(g["weight_decay"])
-        if not grads:
-            return loss
-        if todo:
-            self._new_states(todo)
-        norm = grad_norm(grads, scale) if self.max_norm is not None else None
-        for r, (key, (ps, sts, lrs, wds, lr)) in enumerate(runs.items()):
-            ms, vs, ts = zip(*(self._moments(st) for st in sts)) if ps else ((), (), ())
+            grads = [p.grad for p in ps]
+            states = self._states(ps, grads)
+            if key not in runs:
+                runs[key] = ([], [], [], [], [], [], [])
+            for l, more in zip(runs[key], (ps, grads, *states, [lr] * len(ps), [g["weight_decay"]] * len(ps))):
+                l += more
+        norm = grad_norm([g for run in runs.values() for g in run[1]], scale) if self.max_norm is not None else None
+        if norm is not None and not norm.is_cuda:
+            return loss                                    # no gradients at all
+        for r, (key, (ps, grads, ms, vs, ts, lrs, wds)) in enumerate(runs.items()):
             # the seeds of several runs differ, so that their roundings do not repeat one another's
-            adamw_step(ps, [p.grad for p in ps], ms, vs, ts, lr=lr if torch.is_tensor(lr) else lrs, betas=key[0], eps=key[1],
-                       weight_decay=wds, maximize=key[2], seed=self.seed + 0x51F15EED * r, total_norm=norm,
-                       max_norm=self.max_norm if norm is not None else None, grad_scale=scale, found_inf=found)
+            adamw_step(ps, grads, ms, vs, ts, lr=lrs[0] if key[3] >= 0 and lrs else lrs, betas=key[0], eps=key[1], weight_decay=wds,
+                       maximize=key[2], seed=self.seed + 0x51F15EED * r, total_norm=norm, max_norm=self.max_norm, grad_scale=scale,
+                       found_inf=found)
         return loss
 
     def load_state_dict(self, state_dict):
