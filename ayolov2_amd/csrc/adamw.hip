@@ -8,9 +8,9 @@
 //
 // Bound: HBM.  Per fp32 parameter 4 B for the norm, 8 B for the clipping, 28 B for AdamW with 32-bit moments and 16 B with 8-bit
 // ones.  The tensors come as a list on the host and travel BY VALUE in the kernel arguments (up to 4 KB per launch), so nothing is
-// copied to the device, nothing has to be kept between calls, and a captured call replays as it is.  An address is kept as a
-// 32-bit distance from the launch's first tensor, so that a launch takes 330 gradients, 160 tensors with 32-bit and 120 with 8-bit
-// moments: every further launch costs some 4 us of start and drain.
+// copied to the device, nothing has to be kept between calls, and a captured call replays as it is.  An address is kept as its low
+// half and the number of its 4 GB window, of which a launch knows 16 (an allocator's segments lie far apart), so that a launch
+// takes 240 gradients, 140 tensors with 32-bit and 110 with 8-bit moments: every further launch costs some 4 us of start and drain.
 // A workgroup takes CHUNK elements of one tensor; it finds its tensor by comparing the jobs' first workgroups 64 at a time.
 #include "common.h"
 #include <math.h>
@@ -84,21 +84,39 @@ __device__ __forceinline__ void each_part(unsigned at, unsigned n, F f) {
     for (unsigned i = at; i < at + CHUNK && i < n; i += 1024) f(i);
 }
 
-// A launch's tensors.  HEAD: what the kernel needs besides; N addresses per tensor, each in steps of its own unit.
+// A launch's tensors.  HEAD: what the kernel needs besides; N addresses per tensor.
 struct Where { unsigned first, tag, tensor; };             // first workgroup; two bits of the caller's; place in the caller's list
+// 4 GB windows of addresses: the high halves, by number
+struct Windows {
+    static constexpr int MAX = 16;
+    unsigned hi[MAX];
+    // (through the global address space: an address made of numbers would be taken for a generic one)
+    __device__ __forceinline__ void* at(unsigned which, unsigned lo) const {
+        return (void*)(__attribute__((address_space(1))) void*)((uint64_t)hi[which] << 32 | lo);
+    }
+    // host: the number of an address's window among the first `n`, added where it is new; -1: no room
+    int number(int& n, const void* p) {
+        const unsigned h = (unsigned)((uintptr_t)p >> 32);
+        for (int k = 0; k < n; ++k)
+            if (hi[k] == h) return k;
+        if (n == MAX) return -1;
+        hi[n] = h;
+        return n++;
+    }
+};
 template <typename HEAD, int N> struct Jobs {
     static constexpr int ADDRESSES = N;
     struct Job {
-        int off[N];
+        unsigned lo[N], windows;                           // four bits of window per address
         unsigned n, meta;                                  // elements; first workgroup (21 bits), tag (2), place (9)
     };
-    static constexpr int MAX = (4096 - (int)sizeof(HEAD) - 8 * N - 16) / (int)sizeof(Job);
+    static constexpr int MAX = (4096 - (int)sizeof(HEAD) - (int)sizeof(Windows) - 16) / (int)sizeof(Job);
     HEAD h;
-    char* base[N];
+    Windows w;
     int njobs;
     unsigned tensor0;
     Job j[MAX];
-    template <typename T> __device__ __forceinline__ T* at(int k, int a, int unit = sizeof(T)) const { return (T*)(base[a] + (int64_t)j[k].off[a] * unit); }
+    template <typename T> __device__ __forceinline__ T* at(int k, int a) const { return (T*)w.at(j[k].windows >> 4 * a & 15u, j[k].lo[a]); }
     __device__ __forceinline__ Where where(int k) const {
         const unsigned m = j[k].meta;
         return Where{m & 0x1fffffu, m >> 21 & 3u, tensor0 + (m >> 23)};
@@ -119,7 +137,7 @@ struct GHead {
     double* part;
     float max_norm;
 };
-typedef Jobs<GHead, 1> GJobs;                              // tag: the gradient's type; unit: 2 bytes
+typedef Jobs<GHead, 1> GJobs;                              // tag: the gradient's type
 static_assert(sizeof(GJobs) <= 4096, "kernel arguments");
 
 template <bool FULL, typename T>
@@ -151,9 +169,9 @@ __global__ __launch_bounds__(256) void k_grad_squares(GJobs P) {
         each_part(at, n, [&](unsigned i) { t += squares<false>(g, n, i); });
         return t;
     };
-    double s = J.tag == AYOLO_F32   ? of(P.at<const float>(j, 0, 2))
-               : J.tag == AYOLO_F16 ? of(P.at<const half_t>(j, 0, 2))
-                                    : of(P.at<const bf16_t>(j, 0, 2));
+    double s = J.tag == AYOLO_F32   ? of(P.at<const float>(j, 0))
+               : J.tag == AYOLO_F16 ? of(P.at<const half_t>(j, 0))
+                                    : of(P.at<const bf16_t>(j, 0));
     s = wave_sum(s);
     if ((threadIdx.x & 63) == 0) w[threadIdx.x >> 6] = s;
     __syncthreads();
@@ -197,9 +215,9 @@ __global__ __launch_bounds__(256) void k_grad_clip(GJobs P) {
         if (at + CHUNK <= n) scale<true>(g, n, at, f);
         else each_part(at, n, [&](unsigned i) { scale<false>(g, n, i, f); });
     };
-    if (J.tag == AYOLO_F32) of(P.at<float>(j, 0, 2));
-    else if (J.tag == AYOLO_F16) of(P.at<half_t>(j, 0, 2));
-    else of(P.at<bf16_t>(j, 0, 2));
+    if (J.tag == AYOLO_F32) of(P.at<float>(j, 0));
+    else if (J.tag == AYOLO_F16) of(P.at<half_t>(j, 0));
+    else of(P.at<bf16_t>(j, 0));
 }
 
 // -------------------------------------------------------------------------------------------------- 8-bit moments
@@ -325,15 +343,15 @@ struct Coef { float step, decay, root; unsigned key; };    // lr / (1 - b1^t), l
 
 // Tensors that share a learning rate and decay share an entry of `pair`.
 struct PrepJobs {
-    static constexpr int MAX = 430, PAIRS = 64;
+    static constexpr int MAX = 420, PAIRS = 64;
     double ln_b1, ln_b2;
     const float *lr, *found_inf;
     Coef* out;
-    char* step;
     unsigned seed, place0;
     int n, pairs;
+    Windows w;
     struct { float lr, wd; } pair[PAIRS];
-    struct { int off; unsigned which; } j[MAX];            // the step count's place; pair (6 bits), place in the list - place0 (26)
+    struct { unsigned lo, which; } j[MAX];                 // the step count's address; pair (6 bits), window (4), place in the list - place0 (22)
 };
 static_assert(sizeof(PrepJobs) <= 4096, "kernel arguments");
 
@@ -343,8 +361,8 @@ __global__ __launch_bounds__(512) void k_adamw_prepare(PrepJobs P) {
     const int i = threadIdx.x;
     if (i >= P.n) return;
     if (P.found_inf && *P.found_inf != 0.0f) return;
-    float* step = (float*)(P.step + (int64_t)P.j[i].off * 4);
-    const unsigned pair = P.j[i].which & 63u, place = P.place0 + (P.j[i].which >> 6);
+    float* step = (float*)P.w.at(P.j[i].which >> 6 & 15u, P.j[i].lo);
+    const unsigned pair = P.j[i].which & 63u, place = P.place0 + (P.j[i].which >> 10);
     const float t = *step + 1.0f;
     *step = t;
     const double lr = P.lr ? (double)*P.lr : (double)P.pair[pair].lr;
@@ -575,32 +593,42 @@ struct Ranges {
 // Splits a list into launches.  where(i, off, address): a job's addresses, from element `off` of tensor i on; tag(i, part): its two
 // bits; go(jobs, workgroups) launches what has gathered.
 template <typename JOBS, typename WHERE, typename TAG, typename GO>
-int each_launch(JOBS& P, const ayolo_tensor* t, int n, const int (&unit)[JOBS::ADDRESSES], WHERE where, TAG tag, GO go) {
+int each_launch(JOBS& P, const ayolo_tensor* t, int n, WHERE where, TAG tag, GO go) {
+    constexpr int N = JOBS::ADDRESSES;
+    static_assert(N <= 8, "four bits of window per address");
     unsigned wgs = 0;
+    int windows = 0;
     P.njobs = 0;
     auto flush = [&]() -> int {
         const int rc = P.njobs ? go(P, wgs) : AYOLO_OK;
-        P.njobs = 0;
+        P.njobs = windows = 0;
         wgs = 0;
         return rc;
     };
     for (int i = 0; i < n; ++i) {
         if (!t[i].present) continue;
         for (int64_t off = 0; off < t[i].numel; off += PART) {
-            char* a[JOBS::ADDRESSES];
+            char* a[N];
             where(i, off, a);
-            bool fits = P.njobs > 0 && P.njobs < JOBS::MAX && wgs < MOST_WGS && (unsigned)i - P.tensor0 < 512u;
-            for (int k = 0; k < JOBS::ADDRESSES && fits; ++k) {
-                const int64_t d = (int64_t)((uintptr_t)a[k] - (uintptr_t)P.base[k]) / unit[k];
-                fits = d >= INT32_MIN && d <= INT32_MAX;
-            }
-            if (!fits) {
+            unsigned which = 0;
+            auto fits = [&]() {
+                if (P.njobs == JOBS::MAX || wgs >= MOST_WGS || (P.njobs && (unsigned)i - P.tensor0 >= 512u)) return false;
+                which = 0;
+                for (int k = 0; k < N; ++k) {
+                    const int w = P.w.number(windows, a[k]);
+                    if (w < 0) return false;
+                    which |= (unsigned)w << 4 * k;
+                }
+                return true;
+            };
+            if (!fits()) {
                 if (const int rc = flush()) return rc;
-                for (int k = 0; k < JOBS::ADDRESSES; ++k) P.base[k] = a[k];
-                P.tensor0 = (unsigned)i;
+                fits();                                    // alone it does: N windows at most
             }
+            if (P.njobs == 0) P.tensor0 = (unsigned)i;
             auto& J = P.j[P.njobs++];
-            for (int k = 0; k < JOBS::ADDRESSES; ++k) J.off[k] = (int)((int64_t)((uintptr_t)a[k] - (uintptr_t)P.base[k]) / unit[k]);
+            for (int k = 0; k < N; ++k) J.lo[k] = (unsigned)(uintptr_t)a[k];
+            J.windows = which;
             J.n = (unsigned)std::min<int64_t>(PART, t[i].numel - off);
             J.meta = wgs | tag(i, (unsigned)(off / PART)) << 21 | ((unsigned)i - P.tensor0) << 23;
             wgs += (J.n + CHUNK - 1) / CHUNK;
@@ -619,7 +647,7 @@ int64_t chunks_of(const ayolo_tensor* t, int n) {
 
 template <typename GO>
 int grad_launches(GJobs& P, const ayolo_tensor* grads, int n, GO go) {
-    return each_launch(P, grads, n, {2}, [&](int i, int64_t off, char** a) { a[0] = (char*)grads[i].data + off * es_of(grads[i].dtype); },
+    return each_launch(P, grads, n, [&](int i, int64_t off, char** a) { a[0] = (char*)grads[i].data + off * es_of(grads[i].dtype); },
                        [&](int i, unsigned) { return (unsigned)grads[i].dtype; }, go);
 }
 
@@ -706,10 +734,7 @@ int adamw_launches(const ayolo_adamw_list& L, const Hyper& h, hipStream_t s) {
         };
         auto part = [](int, unsigned p) { return p & 3u; };
         P.h.coef = h.coef + from;
-        int rc;
-        if constexpr (BITS8) rc = each_launch(P, L.g + from, to - from, {es, es, 1, 1, 1, 1}, where, part, go);
-        else rc = each_launch(P, L.g + from, to - from, {es, es, 4, 4}, where, part, go);
-        if (rc) return rc;
+        if (const int rc = each_launch(P, L.g + from, to - from, where, part, go)) return rc;
         from = to;
     }
     return AYOLO_OK;
@@ -777,33 +802,35 @@ extern "C" int ayolo_adamw_step(const ayolo_adamw_list* L, const ayolo_adamw_hyp
     Q.found_inf = H->found_inf;
     Q.out = (Coef*)ws;
     Q.seed = H->seed;
+    int windows = 0;
     auto prepare = [&]() -> int {
         if (Q.n == 0) return AYOLO_OK;
         hipLaunchKernelGGL(k_adamw_prepare, dim3(1), dim3(512), 0, s, Q);
         AY_CHECK_LAUNCH("k_adamw_prepare");
-        Q.n = 0;
+        Q.n = Q.pairs = windows = 0;
         return AYOLO_OK;
     };
     for (int i = 0; i < n; ++i) {
         if (!L->g[i].present) continue;
         const float lr = L->lr ? L->lr[i] : H->lr, wd = L->weight_decay ? L->weight_decay[i] : H->weight_decay;
-        int pair = 0;
-        if (Q.n)
-            while (pair < Q.pairs && !(Q.pair[pair].lr == lr && Q.pair[pair].wd == wd)) ++pair;
-        const int64_t d = Q.n ? (int64_t)((uintptr_t)L->step[i].data - (uintptr_t)Q.step) / 4 : 0;
-        if (Q.n == 0 || Q.n == PrepJobs::MAX || pair == PrepJobs::PAIRS || d < INT32_MIN || d > INT32_MAX || (unsigned)i - Q.place0 >= 1u << 26) {
+        int pair = 0, w = 0;
+        auto fits = [&]() {
+            if (Q.n == PrepJobs::MAX || (Q.n && (unsigned)i - Q.place0 >= 1u << 22)) return false;
+            for (pair = 0; pair < Q.pairs && !(Q.pair[pair].lr == lr && Q.pair[pair].wd == wd);) ++pair;
+            return pair < PrepJobs::PAIRS && (w = Q.w.number(windows, L->step[i].data)) >= 0;
+        };
+        if (!fits()) {
             if (const int rc = prepare()) return rc;
-            Q.step = (char*)L->step[i].data;
-            Q.place0 = (unsigned)i;
-            Q.pairs = pair = 0;
+            fits();
         }
+        if (Q.n == 0) Q.place0 = (unsigned)i;
         if (pair == Q.pairs) {
             Q.pair[pair].lr = lr;
             Q.pair[pair].wd = wd;
             ++Q.pairs;
         }
-        Q.j[Q.n].off = (int)((int64_t)((uintptr_t)L->step[i].data - (uintptr_t)Q.step) / 4);
-        Q.j[Q.n].which = (unsigned)pair | ((unsigned)i - Q.place0) << 6;
+        Q.j[Q.n].lo = (unsigned)(uintptr_t)L->step[i].data;
+        Q.j[Q.n].which = (unsigned)pair | (unsigned)w << 6 | ((unsigned)i - Q.place0) << 10;
         ++Q.n;
     }
     if (const int rc = prepare()) return rc;
@@ -835,7 +862,7 @@ extern "C" int ayolo_moment_values(const ayolo_tensor* codes, const ayolo_tensor
     }
     hipStream_t s = (hipStream_t)st;
     UJobs P{};
-    return each_launch(P, codes, n, {1, 1, 4},
+    return each_launch(P, codes, n,
         [&](int i, int64_t off, char** a) {
             a[0] = (char*)codes[i].data + off;
             a[1] = (char*)exps[i].data + off / 128;
