@@ -11,7 +11,7 @@
 // copied to the device, nothing has to be kept between calls, and a captured call replays as it is.  An address is kept as its low
 // half and the number of its 4 GB window, of which a launch knows 16 (an allocator's segments lie far apart), so that a launch
 // takes 240 gradients, 140 tensors with 32-bit and 110 with 8-bit moments: every further launch costs some 4 us of start and drain.
-// A workgroup takes CHUNK elements of one tensor; it finds its tensor by comparing the jobs' first workgroups 64 at a time.
+// A workgroup takes a chunk of one tensor; it finds its tensor by comparing the jobs' first workgroups 64 at a time.
 #include "common.h"
 #include <math.h>
 #include <algorithm>
@@ -22,9 +22,13 @@ typedef unsigned v2u __attribute__((ext_vector_type(2)));
 
 namespace {
 
-constexpr int CHUNK = 4096;                                // elements per workgroup: 256 threads x 4 vectors of 4
-constexpr unsigned PART = 1u << 30;                        // a larger tensor travels as several jobs (a multiple of CHUNK)
-constexpr unsigned MOST_WGS = 1u << 20;                    // of a launch, before its last job (at most 2^18 more)
+// Elements per workgroup of 256 threads, as vectors of four that all are loaded before the first is used.  One tensor's chunks
+// are many and short, so that the drain of a launch is short too: 46.5 M bf16 parameters take 169 / 179 / 192 / 206 us with 2048 /
+// 4096 / 8192 / 16384 elements a workgroup, 86.7 M with 8-bit moments 399 / 408 / 442 / 476.  The norm and the clipping, with one
+// vector to load per element, take 104 / 97 / 98 / 99.
+constexpr int CHUNK_ADAMW = 2048, CHUNK_GRAD = 4096, CHUNK_VALUES = 4096;
+constexpr unsigned PART = 1u << 30;                        // a larger tensor travels as several jobs (a multiple of every chunk)
+constexpr unsigned MOST_WGS = 1u << 20;                    // of a launch, before its last job (at most 2^19 more)
 
 template <typename T> struct V4 { typedef T type __attribute__((ext_vector_type(4), aligned(sizeof(T)))); };
 // ONCE: past the caches, for what is not used again before the caches have seen everything else.  The gradients, the moments and
@@ -77,9 +81,9 @@ template <bool FULL> struct At {
         else if (left > 0) store_upto(p + i, v, left);
     }
 };
-// A whole chunk is four vectors per thread at once; the others go one by one (they are few, and the code stays small).
-template <bool FULL> constexpr int U = FULL ? CHUNK / 1024 : 1;
-template <typename F>
+// A whole chunk goes at once; the others go one vector per thread at a time (they are few, and the code stays small).
+template <bool FULL, int CHUNK> constexpr int U = FULL ? CHUNK / 1024 : 1;
+template <int CHUNK, typename F>
 __device__ __forceinline__ void each_part(unsigned at, unsigned n, F f) {
     for (unsigned i = at; i < at + CHUNK && i < n; i += 1024) f(i);
 }
@@ -104,8 +108,8 @@ struct Windows {
         return n++;
     }
 };
-template <typename HEAD, int N> struct Jobs {
-    static constexpr int ADDRESSES = N;
+template <typename HEAD, int N, int CH> struct Jobs {
+    static constexpr int ADDRESSES = N, CHUNK = CH;
     struct Job {
         unsigned lo[N], windows;                           // four bits of window per address
         unsigned n, meta;                                  // elements; first workgroup (21 bits), tag (2), place (9)
@@ -137,17 +141,17 @@ struct GHead {
     double* part;
     float max_norm;
 };
-typedef Jobs<GHead, 1> GJobs;                              // tag: the gradient's type
+typedef Jobs<GHead, 1, CHUNK_GRAD> GJobs;                              // tag: the gradient's type
 static_assert(sizeof(GJobs) <= 4096, "kernel arguments");
 
 template <bool FULL, typename T>
 __device__ __forceinline__ double squares(const T* g, unsigned n, unsigned at) {
-    float4v x[U<FULL>];
+    float4v x[U<FULL, CHUNK_GRAD>];
 #pragma unroll
-    for (int k = 0; k < U<FULL>; ++k) x[k] = At<FULL>(at, k, n).load(g);
+    for (int k = 0; k < U<FULL, CHUNK_GRAD>; ++k) x[k] = At<FULL>(at, k, n).load(g);
     double s = 0.0;
 #pragma unroll
-    for (int k = 0; k < U<FULL>; ++k)
+    for (int k = 0; k < U<FULL, CHUNK_GRAD>; ++k)
 #pragma unroll
         for (int e = 0; e < 4; ++e) s += (double)x[k][e] * (double)x[k][e];
     return s;
@@ -162,11 +166,11 @@ __global__ __launch_bounds__(256) void k_grad_squares(GJobs P) {
     __shared__ double w[4];
     const int j = P.mine();
     const Where J = P.where(j);
-    const unsigned at = (blockIdx.x - J.first) * CHUNK, n = P.j[j].n;
+    const unsigned at = (blockIdx.x - J.first) * CHUNK_GRAD, n = P.j[j].n;
     auto of = [&](auto* g) {
-        if (at + CHUNK <= n) return squares<true>(g, n, at);
+        if (at + CHUNK_GRAD <= n) return squares<true>(g, n, at);
         double t = 0.0;
-        each_part(at, n, [&](unsigned i) { t += squares<false>(g, n, i); });
+        each_part<CHUNK_GRAD>(at, n, [&](unsigned i) { t += squares<false>(g, n, i); });
         return t;
     };
     double s = J.tag == AYOLO_F32   ? of(P.at<const float>(j, 0))
@@ -180,7 +184,14 @@ __global__ __launch_bounds__(256) void k_grad_squares(GJobs P) {
 __global__ __launch_bounds__(1024) void k_grad_norm(const double* part, int64_t n, const float* grad_scale, float* out) {
     __shared__ double w[16];
     double s = 0.0;
-    for (int64_t i = threadIdx.x; i < n; i += 1024) s += part[i];
+    int64_t i = threadIdx.x;
+    for (; i + 7 * 1024 < n; i += 8 * 1024) {              // eight loads in flight
+        double v[8];
+#pragma unroll
+        for (int k = 0; k < 8; ++k) v[k] = part[i + 1024 * k];
+        s += ((v[0] + v[1]) + (v[2] + v[3])) + ((v[4] + v[5]) + (v[6] + v[7]));
+    }
+    for (; i < n; i += 1024) s += part[i];
     s = wave_sum(s);
     if ((threadIdx.x & 63) == 0) w[threadIdx.x >> 6] = s;
     __syncthreads();
@@ -200,20 +211,20 @@ __device__ __forceinline__ float clip_factor(const float* norm, float max_norm) 
 
 template <bool FULL, typename T>
 __device__ __forceinline__ void scale(T* g, unsigned n, unsigned at, float f) {
-    float4v x[U<FULL>];
+    float4v x[U<FULL, CHUNK_GRAD>];
 #pragma unroll
-    for (int k = 0; k < U<FULL>; ++k) x[k] = At<FULL>(at, k, n).template load<true>(g);
+    for (int k = 0; k < U<FULL, CHUNK_GRAD>; ++k) x[k] = At<FULL>(at, k, n).template load<true>(g);
 #pragma unroll
-    for (int k = 0; k < U<FULL>; ++k) At<FULL>(at, k, n).template store<true>(g, x[k] * f);
+    for (int k = 0; k < U<FULL, CHUNK_GRAD>; ++k) At<FULL>(at, k, n).template store<true>(g, x[k] * f);
 }
 __global__ __launch_bounds__(256) void k_grad_clip(GJobs P) {
     const int j = P.mine();
     const Where J = P.where(j);
-    const unsigned at = (blockIdx.x - J.first) * CHUNK, n = P.j[j].n;
+    const unsigned at = (blockIdx.x - J.first) * CHUNK_GRAD, n = P.j[j].n;
     const float f = clip_factor(P.h.norm, P.h.max_norm);
     auto of = [&](auto* g) {
-        if (at + CHUNK <= n) scale<true>(g, n, at, f);
-        else each_part(at, n, [&](unsigned i) { scale<false>(g, n, i, f); });
+        if (at + CHUNK_GRAD <= n) scale<true>(g, n, at, f);
+        else each_part<CHUNK_GRAD>(at, n, [&](unsigned i) { scale<false>(g, n, i, f); });
     };
     if (J.tag == AYOLO_F32) of(P.at<float>(j, 0));
     else if (J.tag == AYOLO_F16) of(P.at<half_t>(j, 0));
@@ -381,7 +392,7 @@ struct Hyper {
     int maximize;
 };
 // p, g, m, v (and the moments' exponents); tag: which 2^30 elements of its tensor a job is
-template <bool BITS8> using AJobs = Jobs<Hyper, BITS8 ? 6 : 4>;
+template <bool BITS8> using AJobs = Jobs<Hyper, BITS8 ? 6 : 4, CHUNK_ADAMW>;
 static_assert(sizeof(AJobs<false>) <= 4096 && sizeof(AJobs<true>) <= 4096, "kernel arguments");
 template <typename T, bool BITS8> struct Tensor;
 template <typename T> struct Tensor<T, false> {
@@ -434,9 +445,9 @@ __device__ __forceinline__ float4v stepped(float4v p, float4v m, float4v v, cons
 
 template <bool FULL, typename T>
 __device__ __forceinline__ void step_chunk(const Tensor<T, false>& J, const Hyper& h, const Coef& c, const Scalars& sc, unsigned at) {
-    float4v x[U<FULL>], d[U<FULL>], m[U<FULL>], v[U<FULL>];
+    float4v x[U<FULL, CHUNK_ADAMW>], d[U<FULL, CHUNK_ADAMW>], m[U<FULL, CHUNK_ADAMW>], v[U<FULL, CHUNK_ADAMW>];
 #pragma unroll
-    for (int k = 0; k < U<FULL>; ++k) {
+    for (int k = 0; k < U<FULL, CHUNK_ADAMW>; ++k) {
         const At<FULL> a(at, k, J.n);
         d[k] = a.template load<true>(J.g);
         m[k] = a.template load<true>(J.m);
@@ -444,7 +455,7 @@ __device__ __forceinline__ void step_chunk(const Tensor<T, false>& J, const Hype
         x[k] = a.template load<true>(J.p);
     }
 #pragma unroll
-    for (int k = 0; k < U<FULL>; ++k) {
+    for (int k = 0; k < U<FULL, CHUNK_ADAMW>; ++k) {
         const At<FULL> a(at, k, J.n);
         moments(true_grad(d[k], sc), h, m[k], v[k]);
         a.template store<true>(J.m, m[k]);
@@ -455,11 +466,11 @@ __device__ __forceinline__ void step_chunk(const Tensor<T, false>& J, const Hype
 // 32 lanes hold one block of 128
 template <bool FULL, typename T>
 __device__ __forceinline__ void step_chunk(const Tensor<T, true>& J, const Hyper& h, const Coef& c, const Scalars& sc, unsigned at) {
-    float4v x[U<FULL>], d[U<FULL>];
-    unsigned mc[U<FULL>], vc[U<FULL>];
-    int me[U<FULL>], ve[U<FULL>];
+    float4v x[U<FULL, CHUNK_ADAMW>], d[U<FULL, CHUNK_ADAMW>];
+    unsigned mc[U<FULL, CHUNK_ADAMW>], vc[U<FULL, CHUNK_ADAMW>];
+    int me[U<FULL, CHUNK_ADAMW>], ve[U<FULL, CHUNK_ADAMW>];
 #pragma unroll
-    for (int k = 0; k < U<FULL>; ++k) {
+    for (int k = 0; k < U<FULL, CHUNK_ADAMW>; ++k) {
         const At<FULL> a(at, k, J.n);
         d[k] = a.template load<true>(J.g);
         mc[k] = load_codes(J.m + a.i, a.left);
@@ -469,7 +480,7 @@ __device__ __forceinline__ void step_chunk(const Tensor<T, true>& J, const Hyper
         x[k] = a.template load<true>(J.p);
     }
 #pragma unroll
-    for (int k = 0; k < U<FULL>; ++k) {
+    for (int k = 0; k < U<FULL, CHUNK_ADAMW>; ++k) {
         const At<FULL> a(at, k, J.n);
         float4v m = decode4<true>(mc[k], me[k]), v = decode4<false>(vc[k], ve[k]);
         moments(true_grad(d[k], sc), h, m, v);
@@ -512,35 +523,35 @@ __global__ __launch_bounds__(256) void k_adamw(AJobs<BITS8> P) {
     sc.scaled = h.grad_scale != nullptr;
     sc.scale = sc.scaled ? *h.grad_scale : 1.0f;
     sc.factor = (h.norm ? clip_factor(h.norm, h.max_norm) : 1.0f) * (h.maximize ? -1.0f : 1.0f);
-    const unsigned at = (blockIdx.x - W.first) * CHUNK;
-    if (at + CHUNK <= J.n) step_chunk<true>(J, h, c, sc, at);
-    else each_part(at, J.n, [&](unsigned i) { step_chunk<false>(J, h, c, sc, i); });
+    const unsigned at = (blockIdx.x - W.first) * CHUNK_ADAMW;
+    if (at + CHUNK_ADAMW <= J.n) step_chunk<true>(J, h, c, sc, at);
+    else each_part<CHUNK_ADAMW>(at, J.n, [&](unsigned i) { step_chunk<false>(J, h, c, sc, i); });
 }
 
 struct None {};
-typedef Jobs<None, 3> UJobs;                               // codes, exponents, values
+typedef Jobs<None, 3, CHUNK_VALUES> UJobs;                               // codes, exponents, values
 static_assert(sizeof(UJobs) <= 4096, "kernel arguments");
 template <bool SIGNED, bool FULL>
 __device__ __forceinline__ void values_chunk(const uint8_t* codes, const uint8_t* exps, float* out, unsigned n, unsigned at) {
-    unsigned c[U<FULL>];
-    int e[U<FULL>];
+    unsigned c[U<FULL, CHUNK_VALUES>];
+    int e[U<FULL, CHUNK_VALUES>];
 #pragma unroll
-    for (int k = 0; k < U<FULL>; ++k) {
+    for (int k = 0; k < U<FULL, CHUNK_VALUES>; ++k) {
         const At<FULL> a(at, k, n);
         c[k] = load_codes(codes + a.i, a.left);
         e[k] = exps[a.i / 128];
     }
 #pragma unroll
-    for (int k = 0; k < U<FULL>; ++k) At<FULL>(at, k, n).template store<true>(out, decode4<SIGNED>(c[k], e[k]));
+    for (int k = 0; k < U<FULL, CHUNK_VALUES>; ++k) At<FULL>(at, k, n).template store<true>(out, decode4<SIGNED>(c[k], e[k]));
 }
 template <bool SIGNED>
 __global__ __launch_bounds__(256) void k_moment_values(UJobs P) {
     const int j = P.mine();
-    const unsigned at = (blockIdx.x - P.where(j).first) * CHUNK, n = P.j[j].n;
+    const unsigned at = (blockIdx.x - P.where(j).first) * CHUNK_VALUES, n = P.j[j].n;
     const uint8_t *codes = P.at<const uint8_t>(j, 0), *exps = P.at<const uint8_t>(j, 1);
     float* out = P.at<float>(j, 2);
-    if (at + CHUNK <= n) values_chunk<SIGNED, true>(codes, exps, out, n, at);
-    else each_part(at, n, [&](unsigned i) { values_chunk<SIGNED, false>(codes, exps, out, n, i); });
+    if (at + CHUNK_VALUES <= n) values_chunk<SIGNED, true>(codes, exps, out, n, at);
+    else each_part<CHUNK_VALUES>(at, n, [&](unsigned i) { values_chunk<SIGNED, false>(codes, exps, out, n, i); });
 }
 
 // ------------------------------------------------------------------------------------------------------------- host
@@ -631,7 +642,7 @@ int each_launch(JOBS& P, const ayolo_tensor* t, int n, WHERE where, TAG tag, GO 
             J.windows = which;
             J.n = (unsigned)std::min<int64_t>(PART, t[i].numel - off);
             J.meta = wgs | tag(i, (unsigned)(off / PART)) << 21 | ((unsigned)i - P.tensor0) << 23;
-            wgs += (J.n + CHUNK - 1) / CHUNK;
+            wgs += (J.n + JOBS::CHUNK - 1) / JOBS::CHUNK;
         }
     }
     return flush();
@@ -641,7 +652,7 @@ int64_t chunks_of(const ayolo_tensor* t, int n) {
     int64_t c = 0;
     for (int i = 0; i < n; ++i)
         if (t[i].present)
-            for (int64_t off = 0; off < t[i].numel; off += PART) c += cdiv64(std::min<int64_t>(PART, t[i].numel - off), CHUNK);
+            for (int64_t off = 0; off < t[i].numel; off += PART) c += cdiv64(std::min<int64_t>(PART, t[i].numel - off), CHUNK_GRAD);
     return c;
 }
 
