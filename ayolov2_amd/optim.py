@@ -15,6 +15,7 @@ from __future__ import annotations
 
 import array
 import ctypes
+import numbers
 from typing import NamedTuple, Optional, Sequence, Tuple, Union
 
 import numpy as np
@@ -269,9 +270,9 @@ def unpack_moments(moments: Sequence[Moment8], signed: bool, out: Optional[Seque
 
 def _per_tensor(v, n: int, what: str):
     """(number, None), or (0, n floats as bytes) where a number per tensor is given."""
-    if isinstance(v, (int, float)):
+    if isinstance(v, numbers.Real):
         return float(v), None
-    arr = array.array("f", v)
+    arr = array.array("f", map(float, v))
     if len(arr) != n:
         raise _lib.AyoloError(f"adamw_step: {len(arr)} values of {what} for {n} tensors")
     return 0.0, arr.tobytes()
@@ -440,6 +441,8 @@ class AdamW(torch.optim.AdamW):
         ids = [i for g in state_dict["param_groups"] for i in g["params"]]
         for i, p in zip(ids, (p for g in self.param_groups for p in g["params"])):
             raw = state_dict["state"].get(i)
+            if raw and not p.is_cuda and "exp_avg_exps" in raw:
+                raise _lib.AyoloError("ayolov2_amd.optim.AdamW: 8-bit states need parameters on the GPU")
             if not raw or not p.is_cuda:
                 continue
             st = self.state[p]

@@ -574,6 +574,77 @@ def test_tensors_past_32_bits(bits):
     assert ((g[at].float() - torch.arange(1, len(at) + 1, device="cuda") / 2).abs() <= 2.0 ** -8 * 5).all()
 
 
+def test_tensors_all_over_the_address_space():
+    """Small tensors 5 GB apart, more such places than one launch's list can name."""
+    from ayolov2_amd.optim import adamw_step, clip_grads_, grad_norm, new_moment8, unpack_moments
+    n, blocks = 300, [torch.empty(5 << 30, dtype=torch.uint8, device="cuda") for _ in range(24)]
+    used = [0] * len(blocks)
+
+    def take(k, t):
+        k %= len(blocks)
+        v = blocks[k][used[k]:used[k] + t.numel() * t.element_size()].view(t.dtype)
+        used[k] += 1 << 14
+        v.copy_(t)
+        return v
+
+    host = [[_rand(n + k, torch.float32, 10 * k), _rand(n + k, torch.float32, 10 * k + 1, 0.1)] for k in range(60)]
+    want = float(torch.cat([g for _, g in host]).double().norm())
+    p, g = [take(k, h[0]) for k, h in enumerate(host)], [take(5 * k + 1, h[1]) for k, h in enumerate(host)]
+    m, v, t = ([take(7 * k + j, torch.zeros(n + k)) for k in range(60)] for j in (2, 3, 4))
+    t = [x[:1] for x in t]
+    assert abs(float(grad_norm(g)) - want) <= 2 * U * want
+    adamw_step(p, g, m, v, t, lr=1e-2)
+    m8 = [new_moment8(x) for x in p]
+    adamw_step([x.clone() for x in p], g, m8, [new_moment8(x) for x in p], [torch.zeros((), device="cuda") for _ in p], lr=1e-2)
+    out = unpack_moments(m8, True, [take(11 * k + 3, torch.zeros(n + k)) for k in range(60)])
+    clip_grads_(g, want / 2)
+    for k, (hp, hg) in enumerate(host):
+        wp, wm, wv = ref.adamw(hp, hg, torch.zeros(n + k), torch.zeros(n + k), 1, 1e-2, 0.9, 0.999, 1e-8, 1e-2)
+        assert float(t[k]) == 1.0
+        _check_p(p[k], wp, hp, torch.full_like(wp, 1e-2), torch.float32)
+        assert ((m[k].double().cpu() - wm).abs() <= 4 * U * wm.abs()).all()
+        assert ((out[k].double().cpu() - wm).abs() <= torch.maximum(wm.abs() / 8, wm.abs().max() * 2.0 ** -16)).all()
+        assert ((g[k].double().cpu() - hg.double() / 2).abs() <= 8 * U * hg.double().abs()).all()
+
+
+def test_two_threads_at_once():
+    """Two host threads step two optimisers and run two norms, each on a stream of its own."""
+    import threading
+
+    from ayolov2_amd.functional import layer_norm
+    from ayolov2_amd.optim import AdamW
+
+    def work(seed):
+        ps = _params(seed)
+        x = _rand((500, 33), torch.float32, seed).cuda().requires_grad_()
+        o = AdamW(_groups(ps), lr=1e-2, state_bits=8, max_norm=0.5)
+        _train(o, ps, 8, seed)
+        y = layer_norm(x)
+        return [*ps, y, torch.autograd.grad(y, x, x.detach())[0]]
+
+    want = [work(s) for s in (1, 2)]
+    got, errors = [None, None], []
+
+    def thread(k):
+        try:
+            s = torch.cuda.Stream()
+            with torch.cuda.stream(s):
+                got[k] = work(k + 1)
+            s.synchronize()
+        except Exception as e:  # noqa: BLE001
+            errors.append(e)
+
+    ts = [threading.Thread(target=thread, args=(k,)) for k in range(2)]
+    for t in ts:
+        t.start()
+    for t in ts:
+        t.join()
+    assert not errors, errors
+    for a, b in zip(want, got):
+        for p, q in zip(a, b):
+            assert torch.equal(p, q)
+
+
 def test_the_step_of_a_small_network():
     """Layer norm, its gradients, clipping and the step together: captured replays, eager steps of the framework and float64
     agree; and trainer.training_step clips."""

@@ -249,6 +249,16 @@ def test_adamw_on_the_cpu_is_torchs():
         assert torch.equal(p, q)
 
 
+def test_8_bit_state_dicts_do_not_load_onto_the_cpu():
+    p = torch.nn.Parameter(torch.randn(300))
+    o = optim.AdamW([p])
+    sd = o.state_dict()
+    sd["state"] = {0: {"step": torch.tensor(1.0), "exp_avg": torch.zeros(300, dtype=torch.uint8), "exp_avg_exps": torch.zeros(3, dtype=torch.uint8),
+                       "exp_avg_sq": torch.zeros(300, dtype=torch.uint8), "exp_avg_sq_exps": torch.zeros(3, dtype=torch.uint8)}}
+    with pytest.raises(AyoloError, match="GPU"):
+        o.load_state_dict(sd)
+
+
 def test_adamw_copies_keep_their_settings():
     o = optim.AdamW([torch.nn.Parameter(torch.randn(3))], state_bits=8, max_norm=2.0, seed=5)
     c = copy.deepcopy(o)
