@@ -10,7 +10,7 @@
 // ones.  The tensors come as a list on the host and travel BY VALUE in the kernel arguments (up to 4 KB per launch), so nothing is
 // copied to the device, nothing has to be kept between calls, and a captured call replays as it is.  An address is kept as its low
 // half and the number of its 4 GB window, of which a launch knows 16 (an allocator's segments lie far apart), so that a launch
-// takes 240 gradients, 140 tensors with 32-bit and 110 with 8-bit moments: every further launch costs some 4 us of start and drain.
+// takes 330 gradients, 140 tensors with 32-bit and 110 with 8-bit moments: every further launch costs some 4 us of start and drain.
 // A workgroup takes a chunk of one tensor; it finds its tensor by comparing the jobs' first workgroups 64 at a time.
 #include "common.h"
 #include <math.h>
@@ -108,22 +108,32 @@ struct Windows {
         return n++;
     }
 };
+// a job's numbers: low halves of its addresses, four bits of window for each, elements; first workgroup (21 bits), tag (2), place (9)
+template <int N> struct AddressJob {
+    unsigned lo[N], windows, n, meta;
+    __device__ __forceinline__ unsigned window(int a) const { return windows >> 4 * a & 15u; }
+    __device__ __forceinline__ unsigned place() const { return meta >> 23; }
+    void set(unsigned first, unsigned tag, unsigned at, unsigned w) { meta = first | tag << 21 | at << 23; windows = w; }
+};
+template <> struct AddressJob<1> {                                // a single address and no place: the window takes the place's bits
+    unsigned lo[1], n, meta;
+    __device__ __forceinline__ unsigned window(int) const { return meta >> 23; }
+    __device__ __forceinline__ unsigned place() const { return 0; }
+    void set(unsigned first, unsigned tag, unsigned, unsigned w) { meta = first | tag << 21 | w << 23; }
+};
 template <typename HEAD, int N, int CH> struct Jobs {
     static constexpr int ADDRESSES = N, CHUNK = CH;
-    struct Job {
-        unsigned lo[N], windows;                           // four bits of window per address
-        unsigned n, meta;                                  // elements; first workgroup (21 bits), tag (2), place (9)
-    };
+    typedef AddressJob<N> Job;
     static constexpr int MAX = (4096 - (int)sizeof(HEAD) - (int)sizeof(Windows) - 16) / (int)sizeof(Job);
     HEAD h;
     Windows w;
     int njobs;
     unsigned tensor0;
     Job j[MAX];
-    template <typename T> __device__ __forceinline__ T* at(int k, int a) const { return (T*)w.at(j[k].windows >> 4 * a & 15u, j[k].lo[a]); }
+    template <typename T> __device__ __forceinline__ T* at(int k, int a) const { return (T*)w.at(j[k].window(a), j[k].lo[a]); }
     __device__ __forceinline__ Where where(int k) const {
         const unsigned m = j[k].meta;
-        return Where{m & 0x1fffffu, m >> 21 & 3u, tensor0 + (m >> 23)};
+        return Where{m & 0x1fffffu, m >> 21 & 3u, tensor0 + j[k].place()};
     }
     // the job whose workgroups hold this one (`first` ascends): every `s`-th job first, then the ones behind it
     __device__ __forceinline__ int mine() const {
@@ -584,6 +594,9 @@ struct Ranges {
             if (t[i].present && t[i].numel > 0) r.push_back(R{(uintptr_t)t[i].data, (uintptr_t)t[i].data + (uintptr_t)t[i].numel * es_of(t[i].dtype)});
     }
     bool overlap() {
+        bool ascending = true;
+        for (size_t i = 1; i < r.size() && ascending; ++i) ascending = r[i].from >= r[i - 1].to;
+        if (ascending) return false;
         uintptr_t differ = 0;
         for (const R& x : r) differ |= x.from ^ r[0].from;
         other.resize(r.size());
@@ -639,9 +652,8 @@ int each_launch(JOBS& P, const ayolo_tensor* t, int n, WHERE where, TAG tag, GO 
             if (P.njobs == 0) P.tensor0 = (unsigned)i;
             auto& J = P.j[P.njobs++];
             for (int k = 0; k < N; ++k) J.lo[k] = (unsigned)(uintptr_t)a[k];
-            J.windows = which;
             J.n = (unsigned)std::min<int64_t>(PART, t[i].numel - off);
-            J.meta = wgs | tag(i, (unsigned)(off / PART)) << 21 | ((unsigned)i - P.tensor0) << 23;
+            J.set(wgs, tag(i, (unsigned)(off / PART)), (unsigned)i - P.tensor0, which);
             wgs += (J.n + JOBS::CHUNK - 1) / JOBS::CHUNK;
         }
     }
