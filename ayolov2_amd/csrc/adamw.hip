@@ -115,7 +115,7 @@ template <int N> struct AddressJob {
     __device__ __forceinline__ unsigned place() const { return meta >> 23; }
     void set(unsigned first, unsigned tag, unsigned at, unsigned w) { meta = first | tag << 21 | at << 23; windows = w; }
 };
-template <> struct AddressJob<1> {                                // a single address and no place: the window takes the place's bits
+template <> struct AddressJob<1> {                         // a single address and no place: the window takes the place's bits
     unsigned lo[1], n, meta;
     __device__ __forceinline__ unsigned window(int) const { return meta >> 23; }
     __device__ __forceinline__ unsigned place() const { return 0; }
@@ -151,7 +151,7 @@ struct GHead {
     double* part;
     float max_norm;
 };
-typedef Jobs<GHead, 1, CHUNK_GRAD> GJobs;                              // tag: the gradient's type
+typedef Jobs<GHead, 1, CHUNK_GRAD> GJobs;                  // tag: the gradient's type
 static_assert(sizeof(GJobs) <= 4096, "kernel arguments");
 
 template <bool FULL, typename T>
@@ -232,6 +232,7 @@ __global__ __launch_bounds__(256) void k_grad_clip(GJobs P) {
     const Where J = P.where(j);
     const unsigned at = (blockIdx.x - J.first) * CHUNK_GRAD, n = P.j[j].n;
     const float f = clip_factor(P.h.norm, P.h.max_norm);
+    if (f == 1.0f) return;                                 // nothing to clip: the gradients stay as they are
     auto of = [&](auto* g) {
         if (at + CHUNK_GRAD <= n) scale<true>(g, n, at, f);
         else each_part<CHUNK_GRAD>(at, n, [&](unsigned i) { scale<false>(g, n, i, f); });
@@ -409,8 +410,10 @@ template <typename T> struct Tensor<T, false> {
     T* p;
     const T* g;
     float *m, *v;
-    unsigned n, origin;
-    __device__ __forceinline__ Tensor(const AJobs<false>& P, int j) : p(P.template at<T>(j, 0)), g(P.template at<const T>(j, 1)), m(P.template at<float>(j, 2)), v(P.template at<float>(j, 3)), n(P.j[j].n), origin(0) {}
+    unsigned n;
+    __device__ __forceinline__ Tensor(const AJobs<false>& P, int j)
+        : p(P.template at<T>(j, 0)), g(P.template at<const T>(j, 1)), m(P.template at<float>(j, 2)), v(P.template at<float>(j, 3)),
+          n(P.j[j].n) {}
 };
 template <typename T> struct Tensor<T, true> {
     T* p;
@@ -435,9 +438,10 @@ __device__ __forceinline__ void moments(float4v g, const Hyper& h, float4v& m, f
     v = v * h.b2 + g * g * h.c2;
 }
 // Square root and quotient by the hardware's own functions, each 1 ulp: with the two roundings around them below 4 u of the
-// step.  They take subnormal arguments for zero, which shows where eps is that small too; then the exact functions are used.
+// step.  They may take subnormal numbers for zero: a subnormal v (sqrt below 1.1e-19) is nothing beside an ordinary eps, and for
+// a smaller one the exact functions are used.
 __device__ __forceinline__ float4v stepped(float4v p, float4v m, float4v v, const Coef& c, float eps) {
-    if (eps >= 1e-18f) {
+    if (eps >= 1e-12f) {
 #pragma unroll
         for (int e = 0; e < 4; ++e) {
             const float d = __builtin_fmaf(__builtin_amdgcn_sqrtf(v[e]), c.root, eps);

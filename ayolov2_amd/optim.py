@@ -159,9 +159,11 @@ _TENSOR = np.dtype([("data", "<u8"), ("numel", "<i8"), ("layout", "<u8"), ("dtyp
 MOMENT_BLOCK = 128          # elements of an 8-bit moment that share an exponent
 
 
-def _device_of(tensors, what: str) -> torch.device:
+def _device_of(tensors, what: str) -> Optional[torch.device]:
     for t in tensors:
         if t is not None:
+            if not torch.is_tensor(t):
+                raise _lib.AyoloError(f"{what}: expected a tensor, got {type(t).__name__}")
             if not t.is_cuda:
                 raise _lib.AyoloError(f"{what}: the HIP path needs tensors on the GPU (got {t.device}); there is no CPU fallback")
             return t.device
@@ -223,8 +225,8 @@ def clip_grads_(grads: Sequence[Optional[torch.Tensor]], max_norm: float, norm: 
 
 
 def clip_grad_norm_(parameters, max_norm: float, norm_type: float = 2.0, error_if_nonfinite: bool = False) -> torch.Tensor:
-    """torch.nn.utils.clip_grad_norm_ for the 2-norm: clips the parameters' ``.grad`` in place (three launches per hundred and
-    sixty tensors) and returns their norm.  Gradients on the CPU go to torch's own function."""
+    """torch.nn.utils.clip_grad_norm_ for the 2-norm: clips the parameters' ``.grad`` in place (three launches per 330 tensors;
+    gradients that need no clipping are read once and not written) and returns their norm.  Gradients on the CPU go to torch's own function."""
     if float(norm_type) != 2.0:
         raise _lib.AyoloError(f"clip_grad_norm_: norm_type={norm_type}: only the 2-norm has a kernel")
     parameters = [parameters] if torch.is_tensor(parameters) else list(parameters)

@@ -42,6 +42,8 @@ def test_argument_checks_before_the_gpu():
         optim.clip_grads_([x], float("nan"))
     with pytest.raises(AyoloError, match="2 grads for 1 params"):
         optim.adamw_step([x], [x, x], [x], [x], [x], lr=1e-3)
+    with pytest.raises(AyoloError, match="expected a tensor"):
+        optim.grad_norm([1.0])
     with pytest.raises(AyoloError, match="state_bits"):
         optim.AdamW([torch.nn.Parameter(x)], state_bits=16)
     with pytest.raises(AyoloError, match="max_norm"):
