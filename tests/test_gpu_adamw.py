@@ -646,21 +646,30 @@ def test_two_threads_at_once():
 
 
 def test_the_step_of_a_small_network():
-    """Layer norm, its gradients, clipping and the step together: captured replays, eager steps of the framework and float64
-    agree; and trainer.training_step clips."""
+    """Layer norm, its gradients, clipping and the step together, against float64; and the same steps captured once and replayed
+    against eager ones (32- and 8-bit states)."""
     from ayolov2_amd.functional import layer_norm
     from ayolov2_amd.optim import AdamW
     x = _rand((64, 48), torch.float32, 1).cuda()
     init = [_rand((48, 48), torch.float32, 2, 0.15), torch.ones(48), torch.zeros(48)]
-    a = [torch.nn.Parameter(t.cuda()) for t in init]
-    b = [torch.nn.Parameter(t.double()) for t in init]
+
+    def far(p, q):
+        # an element whose gradient is near zero takes a step of its gradient's rounding's sign: at most 2 lr per step, and few of
+        # them; the others agree to the gradients' rounding (48 terms: 64 u) over v's root
+        d = (p.detach().double().cpu() - q.detach().double().cpu()).abs()
+        return float(d.max()) > 3 * 2 * 1e-2 or float((d > 1e-5).double().mean()) > 0.01
+
+    def step(ps, opt):
+        y, s = layer_norm(x @ ps[0], ps[1], ps[2], residual=x)
+        for p, g in zip(ps, torch.autograd.grad((y * y * y + s).mean(), ps)):
+            p.grad = g
+        opt.step()
+
+    new = lambda: [torch.nn.Parameter(t.cuda()) for t in init]  # noqa: E731
+    a, b = new(), [torch.nn.Parameter(t.double()) for t in init]
     oa, ob = AdamW(a, lr=1e-2, max_norm=1.0), torch.optim.AdamW(b, lr=1e-2)
     for _ in range(3):
-        h = x @ a[0]
-        y, s = layer_norm(h, a[1], a[2], residual=x)
-        (y * y * y + s).mean().backward()
-        oa.step()
-        oa.zero_grad()
+        step(a, oa)
         x64 = x.double().cpu()
         s = x64 @ b[0] + x64
         y = torch.nn.functional.layer_norm(s, (48,), b[1], b[2], 1e-5)
@@ -668,11 +677,29 @@ def test_the_step_of_a_small_network():
         torch.nn.utils.clip_grad_norm_(b, 1.0)
         ob.step()
         ob.zero_grad()
-    for p, q in zip(a, b):
-        # an element whose gradient is near zero takes a step of the gradient's own rounding's sign: at most 2 lr per step, and
-        # few of them; the others agree to the gradients' rounding (48 terms: 64 u) over v's root
-        d = (p.detach().double().cpu() - q.detach()).abs()
-        assert float(d.max()) <= 3 * 2 * 1e-2 and float((d > 1e-5).double().mean()) <= 0.01
+    assert not any(far(p, q) for p, q in zip(a, b))
+    for bits in (32, 8):
+        c, d = new(), new()
+        oc, od = (AdamW(ps, lr=1e-2, max_norm=1.0, state_bits=bits) for ps in (c, d))
+        side = torch.cuda.Stream()
+        side.wait_stream(torch.cuda.current_stream())
+        with torch.cuda.stream(side):
+            step(c, oc)                                    # makes the states and warms the libraries up
+        torch.cuda.current_stream().wait_stream(side)
+        graph = torch.cuda.CUDAGraph()
+        with torch.cuda.graph(graph):
+            step(c, oc)
+        with torch.no_grad():
+            for p, t in zip(c, init):
+                p.copy_(t)
+                for v in oc.state[p].values():
+                    v.zero_()
+        for _ in range(3):
+            graph.replay()
+            step(d, od)
+            torch.cuda.synchronize()
+            assert not any(far(p, q) for p, q in zip(c, d))
+        assert float(oc.state[c[0]]["step"]) == 3.0
 
 
 def test_training_step_clips():
