@@ -180,6 +180,22 @@ def test_adamw_many_tensors_and_skipped_ones():
         _check_p(dev[k][0], wp, host[k][0], torch.full_like(wp, 1e-2), host[k][0].dtype)
 
 
+@pytest.mark.parametrize("bits", [32, 8])
+def test_adamw_a_learning_rate_and_decay_per_tensor(bits):
+    """more different pairs than one prepare launch holds"""
+    from ayolov2_amd.optim import adamw_step, new_moment8
+    n = 150
+    host = [[_rand(100 + k, torch.float32, 2 * k), _rand(100 + k, torch.float32, 2 * k + 1)] for k in range(n)]
+    p, g = [h[0].cuda() for h in host], [h[1].cuda() for h in host]
+    state = (lambda: [new_moment8(x) for x in p]) if bits == 8 else (lambda: [torch.zeros_like(x) for x in p])
+    steps, lrs, wds = torch.zeros(n, device="cuda"), [1e-3 * (k + 1) for k in range(n)], [0.01 * (k % 7) for k in range(n)]
+    adamw_step(p, g, state(), state(), list(steps.unbind()), lr=lrs, weight_decay=wds)
+    assert (steps == 1).all()
+    for k, (hp, hg) in enumerate(host):
+        wp, _, _ = ref.adamw(hp, hg, torch.zeros_like(hp), torch.zeros_like(hp), 1, lrs[k], 0.9, 0.999, 1e-8, wds[k])
+        _check_p(p[k], wp, hp, torch.full_like(wp, lrs[k]), torch.float32)
+
+
 def test_adamw_clipped_scaled_skipped_maximized():
     from ayolov2_amd.optim import adamw_step, grad_norm
     hp, hg = _rand(5000, torch.float32, 1), _rand(5000, torch.float32, 2)

@@ -106,6 +106,13 @@ def test_row_counts(rows, C):
     _check(x, *_params(C, torch.float32, 5), 1e-5, gy=gy)
 
 
+@pytest.mark.parametrize("C", [16392, 33000])
+def test_many_long_rows(C):
+    """rows walked in pieces, more of them than the groups that sum the parameters' gradients"""
+    x, gy = _make((150, C), torch.bfloat16, 1), _make((150, C), torch.bfloat16, 2, 1.0, 0.0)
+    _check(x, *_params(C, torch.bfloat16, 3), 1e-5, r=_make((150, C), torch.bfloat16, 4), gy=gy, gs=_make((150, C), torch.bfloat16, 5))
+
+
 def test_no_rows():
     from ayolov2_amd.functional import layer_norm
     x = torch.empty(0, 16, device="cuda", requires_grad=True)
