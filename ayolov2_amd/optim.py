@@ -270,6 +270,50 @@ def unpack_moments(moments: Sequence[Moment8], signed: bool, out: Optional[Seque
     return out
 
 
+def _layouts(tensors) -> np.ndarray:
+    """A number per tensor that is equal for equal shapes in equal memory order, 0 for what is no dense block of memory."""
+    return np.frombuffer(_lib.tensor_rows(tensors, "memory order"), dtype=_TENSOR)["layout"]
+
+
+def _moment_like(p: torch.Tensor, m: torch.Tensor) -> torch.Tensor:
+    """An fp32 moment in parameter `p`'s memory order."""
+    return torch.empty_like(p, dtype=torch.float32, memory_format=torch.preserve_format).copy_(m)
+
+
+def _moment8_like(p: torch.Tensor, m: Moment8, signed: bool) -> Moment8:
+    """An 8-bit moment in parameter `p`'s memory order.  The exponents belong to blocks of codes in the codes' OWN order: in another
+    one the blocks are others, so the values are taken out and put into codes again."""
+    own, want = _layouts([m[0], p])
+    if own != 0 and own == want:
+        codes = torch.empty_like(p, dtype=torch.uint8, memory_format=torch.preserve_format)
+        return Moment8(codes.copy_(m[0]), m[1])
+    return _pack_moment(_moment_like(p, unpack_moments([m], signed)[0]), signed)
+
+
+def _pack_moment(x: torch.Tensor, signed: bool) -> Moment8:
+    """Fp32 values (a dense block of memory) in 8 bits, by the format of csrc/adamw.hip: the rounding to nearest of one conversion,
+    1/16 of a value at most (a step's own rounding is stochastic because it is repeated; this one is not)."""
+    bias, least, top = (14, 1, 0x7F) if signed else (30, 10, 0xFF)
+    n = x.numel()
+    flat = torch.zeros(-(-n // MOMENT_BLOCK) * MOMENT_BLOCK, device=x.device)
+    flat[:n] = x.as_strided((n,), (1,))
+    flat = flat.view(-1, MOMENT_BLOCK)
+    bits = flat.abs().view(torch.int32)
+    finite = bits < 0x7F800000
+    e = (torch.where(finite, bits, 0).amax(1) >> 23).clamp(min=least) if n else bits.new_zeros(0)
+    power = ((bias - e.long() + 1023) << 52).view(torch.float64)          # 2 ** (bias - e)
+    y = (torch.where(finite, flat.abs(), 0.0).double() * power[:, None]).float()
+    code = (y.view(torch.int32) + 0x80008) >> 20
+    if not signed:
+        code = torch.where(bits != 0, code.clamp(min=1), code)            # above zero stays above zero
+    code = torch.where(finite, code, torch.where(bits == 0x7F800000, top - 1, top))
+    if signed:
+        code = torch.where((flat.view(torch.int32) < 0) & (bits <= 0x7F800000), code | 0x80, code)
+    codes = torch.empty_like(x, dtype=torch.uint8, memory_format=torch.preserve_format)
+    codes.as_strided((n,), (1,)).copy_(code.view(-1)[:n])
+    return Moment8(codes, e.to(torch.uint8))
+
+
 def _per_tensor(v, n: int, what: str):
     """(number, None), or (0, n floats as bytes) where a number per tensor is given."""
     if isinstance(v, numbers.Real):
@@ -453,14 +497,11 @@ class AdamW(torch.optim.AdamW):
                 raise _lib.AyoloError("ayolov2_amd.optim.AdamW: a state dict with 32-bit moments does not load into 8-bit states")
             for name, signed in (("exp_avg", True), ("exp_avg_sq", False)):
                 if "exp_avg_exps" in raw:
-                    codes = torch.empty_like(p, dtype=torch.uint8, memory_format=torch.preserve_format)
-                    codes.copy_(raw[name])
-                    m = Moment8(codes, raw[name + "_exps"].to(p.device, copy=True))
+                    m = Moment8(raw[name].to(p.device, copy=True), raw[name + "_exps"].to(p.device, copy=True))
                     if self.state_bits == 8:
-                        st[name], st[name + "_exps"] = m
+                        st[name], st[name + "_exps"] = _moment8_like(p, m, signed)
                     else:
-                        st[name] = unpack_moments([m], signed)[0]
+                        st[name] = _moment_like(p, unpack_moments([m], signed)[0])
                         st.pop(name + "_exps", None)
                 else:
-                    st[name] = torch.empty_like(p, dtype=torch.float32, memory_format=torch.preserve_format)
-                    st[name].copy_(raw[name])
+                    st[name] = _moment_like(p, raw[name])

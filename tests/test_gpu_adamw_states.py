@@ -1,0 +1,96 @@
+"""States of ``optim.AdamW`` that come from, or get into, another memory order than their parameter's.
+
+An 8-bit moment's exponents belong to blocks of 128 codes in MEMORY order.  Taking it to another order means unpacking it in its
+own order and forming new blocks: exact in 32 bits; in 8 bits each value is rounded once to nearest, i.e. by at most 1/16 of
+itself, or below the normal codes by half a step (2^-17 of its new block's largest value for a first moment; for a second one
+by a step, 2^-32, because a value above zero stays above zero)."""
+import numpy as np
+import pytest
+import torch
+
+from oracle import train_ref as ref
+
+pytestmark = pytest.mark.gpu
+SHAPES = [(64, 32, 3, 3), (40, 24, 3, 1), (7, 5, 3, 3), (130,), (16, 8, 1, 1)]
+ORDERS = {"contiguous": torch.contiguous_format, "channels_last": torch.channels_last}
+
+
+def _rand(shape, seed, scale=1.0):
+    return torch.randn(shape, generator=torch.Generator().manual_seed(seed)) * scale
+
+
+def _in_order(t, order):
+    return t.contiguous(memory_format=ORDERS[order]) if t.dim() == 4 else t
+
+
+def _params(order, seed=0):
+    return [torch.nn.Parameter(_in_order(_rand(s, seed + k, 0.1).cuda(), order)) for k, s in enumerate(SHAPES)]
+
+
+def _copy_params(ps, order):
+    return [torch.nn.Parameter(_in_order(p.detach().clone(memory_format=torch.contiguous_format), order)) for p in ps]
+
+
+def _grads(ps, seed):
+    """gradients whose size differs from input channel to input channel, so that blocks along them have other exponents"""
+    for k, p in enumerate(ps):
+        g = _rand(p.shape, 100 * seed + k, 0.01)
+        if p.dim() == 4:
+            g = g * torch.exp2(torch.arange(p.shape[1]) % 12 - 11.0).view(1, -1, 1, 1)
+        p.grad = torch.empty_like(p).copy_(g)
+
+
+def _steps(opt, ps, n, seed):
+    for k in range(n):
+        _grads(ps, seed + k)
+        opt.step()
+
+
+def _values(st, name):
+    from ayolov2_amd.optim import unpack_moments
+    return unpack_moments([(st[name], st[name + "_exps"])], name == "exp_avg")[0]
+
+
+def _flat(t):
+    """the elements in memory order"""
+    return t.detach().as_strided((t.numel(),), (1,), t.storage_offset()).cpu().numpy()
+
+
+def _repacked(values, codes, exps, signed):
+    """`codes`, `exps` are what `values` (laid out as the codes are) round to, bit for bit, within the stated distance"""
+    x = _flat(values)
+    wc, we = ref.encode(x, np.full(x.size, 0x8000, np.uint32), signed)
+    assert np.array_equal(_flat(codes), wc) and np.array_equal(_flat(exps), we)
+    top = np.repeat(np.pad(np.abs(x), (0, -x.size % 128)).reshape(-1, 128).max(1), 128)[:x.size].astype(np.float64)
+    err = np.abs(ref.decode(wc, we, signed).astype(np.float64) - x)
+    assert (err <= np.maximum(np.abs(x) / 16.0, top * 2.0 ** (-17 if signed else -32))).all()
+
+
+@pytest.mark.parametrize("where", ["cuda", "cpu"])
+@pytest.mark.parametrize("src,dst", [("contiguous", "channels_last"), ("channels_last", "contiguous")])
+def test_8_bit_states_load_into_another_memory_order(src, dst, where):
+    from ayolov2_amd.optim import AdamW
+    a = _params(src)
+    oa = AdamW(a, lr=1e-3, state_bits=8, seed=3)
+    _steps(oa, a, 5, 1)
+    sd = oa.state_dict()
+    if where == "cpu":
+        sd = {"state": {i: {k: t.cpu() for k, t in s.items()} for i, s in sd["state"].items()}, "param_groups": sd["param_groups"]}
+    b, c = _copy_params(a, dst), _copy_params(a, dst)
+    o32, o8 = AdamW(b, lr=1e-3), AdamW(c, lr=1e-3, state_bits=8, seed=3)
+    o32.load_state_dict(sd)
+    o8.load_state_dict(sd)
+    for p, q, r in zip(a, b, c):
+        for name, signed in (("exp_avg", True), ("exp_avg_sq", False)):
+            want = _values(oa.state[p], name)
+            got = o32.state[q][name]
+            assert got.stride() == q.stride() and torch.equal(got, want)
+            codes, exps = o8.state[r][name], o8.state[r][name + "_exps"]
+            assert codes.stride() == r.stride()
+            _repacked(got, codes, exps, signed)
+            if p.stride() == r.stride():                   # nothing to re-lay: the same bytes
+                assert torch.equal(codes, oa.state[p][name]) and torch.equal(exps, oa.state[p][name + "_exps"])
+    # and they go on: the 32-bit optimiser from exactly the values that the 8-bit one held
+    for o, ps in ((o32, b), (o8, c)):
+        _steps(o, ps, 1, 77)
+        assert all(float(o.state[p]["step"]) == 6.0 and torch.isfinite(p).all() for p in ps)

@@ -1,0 +1,50 @@
+"""The states of ``optim.AdamW`` without a GPU: the conversion of fp32 values into 8-bit moments, against the oracle's format."""
+import numpy as np
+import pytest
+import torch
+
+from ayolov2_amd import optim
+from oracle import train_ref as ref
+
+
+def _special(signed):
+    g = torch.Generator().manual_seed(0)
+    x = torch.randn(5, 37, 3, 3, generator=g) * torch.exp2(torch.randint(-60, 8, (5, 37, 1, 1), generator=g).float())
+    x = x if signed else x.abs()
+    v = x.view(-1)
+    v[[3, 700]], v[[4, 701]], v[129:300], v[300:310] = float("nan"), float("inf"), 0.0, 1e-42
+    v[310], v[311] = 3.0e38, 2.0 ** -126
+    if signed:
+        v[5], v[6], v[312] = float("-inf"), -0.0, -3.0e38
+    return x
+
+
+@pytest.mark.parametrize("signed", [True, False])
+@pytest.mark.parametrize("order", [torch.contiguous_format, torch.channels_last], ids=["contiguous", "channels_last"])
+def test_packed_as_the_format_says(signed, order):
+    """Bit for bit what the oracle makes of the values in memory order, rounding to nearest (the random number at its middle)."""
+    x = _special(signed).contiguous(memory_format=order)
+    m = optim._pack_moment(x, signed)
+    assert m.codes.stride() == x.stride() and m.codes.dtype == m.exps.dtype == torch.uint8
+    flat = lambda t: t.as_strided((t.numel(),), (1,)).numpy()  # noqa: E731
+    codes, exps = ref.encode(flat(x), np.full(x.numel(), 0x8000, np.uint32), signed)
+    assert np.array_equal(flat(m.codes), codes) and np.array_equal(m.exps.numpy(), exps)
+    back = ref.decode(codes, exps, signed)
+    assert np.array_equal(np.isnan(back), np.isnan(flat(x)))
+    ok = np.isfinite(flat(x)) & (np.abs(flat(x)) < 3e38)
+    top = np.where(np.isfinite(flat(x)), np.abs(flat(x)), 0)
+    top = np.repeat(np.pad(top, (0, -top.size % 128)).reshape(-1, 128).max(1), 128)[:top.size].astype(np.float64)
+    # half a step: 2^-4 of the value, 2^-17 of the block's largest below the normal codes (a second moment never becomes zero: a
+    # step of 2^-32), and the spacing under the least exponents at the bottom of fp32's range
+    tol = np.maximum(np.maximum(np.abs(flat(x).astype(np.float64)) / 16, top * 2.0 ** (-17 if signed else -32)), 2.0 ** -142)
+    assert (np.abs(back[ok].astype(np.float64) - flat(x)[ok]) <= tol[ok]).all()
+    if not signed:
+        assert (back[ok & (flat(x) > 0)] > 0).all()
+
+
+@pytest.mark.parametrize("n", [0, 1, 127, 128, 129])
+def test_packed_sizes(n):
+    x = torch.randn(n, generator=torch.Generator().manual_seed(n))
+    m = optim._pack_moment(x, True)
+    assert m.codes.shape == (n,) and m.exps.shape == (-(-n // 128),)
+    assert (np.abs(ref.decode(m.codes.numpy(), m.exps.numpy(), True) - x.numpy()) <= np.maximum(np.abs(x.numpy()) / 16, 5 * 2.0 ** -17)).all()
