@@ -481,20 +481,52 @@ class AdamW(torch.optim.AdamW):
                        found_inf=found)
         return loss
 
+    def _check_states(self, state_dict) -> None:
+        """Refuses a state dict whose states do not fit this optimiser's parameters."""
+        groups = state_dict["param_groups"]
+        if [len(g["params"]) for g in groups] != [len(g["params"]) for g in self.param_groups]:
+            return                                         # the base class says what is wrong
+        params = [p for g in self.param_groups for p in g["params"]]
+        for i, p in zip((i for g in groups for i in g["params"]), params):
+            raw = state_dict["state"].get(i)
+            if not raw:
+                continue
+            what = f"ayolov2_amd.optim.AdamW: the state of parameter {i}"
+            bits8 = "exp_avg_exps" in raw
+            if bits8 and not p.is_cuda:
+                raise _lib.AyoloError("ayolov2_amd.optim.AdamW: 8-bit states need parameters on the GPU")
+            if not p.is_cuda:
+                continue
+            if self.state_bits == 8 and not bits8:
+                raise _lib.AyoloError("ayolov2_amd.optim.AdamW: a state dict with 32-bit moments does not load into 8-bit states")
+            for name in ("step", "exp_avg", "exp_avg_sq", *(("exp_avg_exps", "exp_avg_sq_exps") if bits8 else ())):
+                if name not in raw:
+                    raise _lib.AyoloError(f"{what} has no {name}")
+            if torch.as_tensor(raw["step"]).numel() != 1:
+                raise _lib.AyoloError(f"{what}: step is not one number")
+            for name in ("exp_avg", "exp_avg_sq"):
+                m = raw[name]
+                if not torch.is_tensor(m) or m.shape != p.shape:
+                    raise _lib.AyoloError(f"{what}: {name} is not a tensor of the parameter's shape {tuple(p.shape)}")
+                if not bits8:
+                    continue
+                e = raw[name + "_exps"]
+                if m.dtype != torch.uint8 or _layouts([m])[0] == 0:
+                    raise _lib.AyoloError(f"{what}: {name} is not a dense block of 8-bit codes")
+                if not torch.is_tensor(e) or e.dtype != torch.uint8 or e.shape != (-(-p.numel() // MOMENT_BLOCK),):
+                    raise _lib.AyoloError(f"{what}: {name}_exps is not one byte per {MOMENT_BLOCK} codes")
+
     def load_state_dict(self, state_dict):
+        self._check_states(state_dict)                     # before anything has changed
         super().load_state_dict(state_dict)
         # the base class has cast every state to its parameter's type: take them again as they were saved
         ids = [i for g in state_dict["param_groups"] for i in g["params"]]
         for i, p in zip(ids, (p for g in self.param_groups for p in g["params"])):
             raw = state_dict["state"].get(i)
-            if raw and not p.is_cuda and "exp_avg_exps" in raw:
-                raise _lib.AyoloError("ayolov2_amd.optim.AdamW: 8-bit states need parameters on the GPU")
             if not raw or not p.is_cuda:
                 continue
             st = self.state[p]
             st["step"] = torch.as_tensor(raw["step"], dtype=torch.float32).detach().reshape(()).to(p.device, copy=True)
-            if self.state_bits == 8 and "exp_avg_exps" not in raw:
-                raise _lib.AyoloError("ayolov2_amd.optim.AdamW: a state dict with 32-bit moments does not load into 8-bit states")
             for name, signed in (("exp_avg", True), ("exp_avg_sq", False)):
                 if "exp_avg_exps" in raw:
                     m = Moment8(raw[name].to(p.device, copy=True), raw[name + "_exps"].to(p.device, copy=True))

@@ -94,3 +94,38 @@ def test_8_bit_states_load_into_another_memory_order(src, dst, where):
     for o, ps in ((o32, b), (o8, c)):
         _steps(o, ps, 1, 77)
         assert all(float(o.state[p]["step"]) == 6.0 and torch.isfinite(p).all() for p in ps)
+
+
+def _changed(sd, **state):
+    """the state dict with entries of its first parameter's state replaced, or taken out (None)"""
+    st = {k: v for k, v in {**sd["state"][0], **state}.items() if v is not None}
+    return {"state": {**sd["state"], 0: st}, "param_groups": [{**g, "lr": 7.0} for g in sd["param_groups"]]}
+
+
+@pytest.mark.parametrize("bits", [32, 8])
+def test_refused_loads_change_nothing(bits):
+    from ayolov2_amd._lib import AyoloError
+    from ayolov2_amd.optim import AdamW
+    ps = _params("channels_last")
+    o = AdamW(ps, lr=1e-3, state_bits=bits)
+    _steps(o, ps, 2, 1)
+    other = AdamW(_copy_params(ps, "channels_last"), lr=1e-3, state_bits=40 - bits)
+    _steps(other, other.param_groups[0]["params"], 1, 9)
+    before = [{k: v.clone() for k, v in o.state[p].items()} for p in ps]
+    sd, n = o.state_dict(), ps[0].numel()
+    bad = [(_changed(sd, exp_avg=sd["state"][0]["exp_avg"][:1]), "shape"), (_changed(sd, exp_avg_sq=None), "no exp_avg_sq"),
+           (_changed(sd, step=torch.zeros(2)), "one number")]
+    if bits == 8:
+        bytes_ = lambda *s: torch.zeros(*s, dtype=torch.uint8, device="cuda")  # noqa: E731
+        bad += [(other.state_dict(), "does not load"), (_changed(sd, exp_avg_exps=bytes_(n // 128 + 1)), "one byte"),
+                (_changed(sd, exp_avg_exps=torch.zeros(n // 128, device="cuda")), "one byte"), (_changed(sd, exp_avg_sq_exps=None), "no exp_avg_sq_exps"),
+                (_changed(sd, exp_avg=torch.zeros(ps[0].shape, device="cuda")), "codes"),
+                (_changed(sd, exp_avg=bytes_(*ps[0].shape, 2)[..., 0]), "dense")]
+    for d, text in bad:
+        with pytest.raises(AyoloError, match=text):
+            o.load_state_dict(d)
+        assert all(g["lr"] == 1e-3 for g in o.param_groups)
+        for p, st in zip(ps, before):
+            assert set(o.state[p]) == set(st)
+            for k, v in st.items():
+                assert o.state[p][k].dtype == v.dtype and torch.equal(o.state[p][k], v)

@@ -4,6 +4,7 @@ import pytest
 import torch
 
 from ayolov2_amd import optim
+from ayolov2_amd._lib import AyoloError
 from oracle import train_ref as ref
 
 
@@ -48,3 +49,29 @@ def test_packed_sizes(n):
     m = optim._pack_moment(x, True)
     assert m.codes.shape == (n,) and m.exps.shape == (-(-n // 128),)
     assert (np.abs(ref.decode(m.codes.numpy(), m.exps.numpy(), True) - x.numpy()) <= np.maximum(np.abs(x.numpy()) / 16, 5 * 2.0 ** -17)).all()
+
+
+def _adamw(device="cpu"):
+    p = torch.nn.Parameter(torch.ones(300, device=device))
+    o = optim.AdamW([p], lr=0.5)
+    p.grad = torch.ones_like(p)
+    return o, p
+
+
+def test_refused_loads_change_nothing():
+    """8-bit states are refused on the CPU, and the optimiser is as it was: settings and states"""
+    o, p = _adamw()
+    o.step()
+    before = {k: v.clone() for k, v in o.state[p].items()}
+    sd = o.state_dict()
+    sd = {"state": {0: {"step": torch.tensor(9.0), "exp_avg": torch.zeros(300, dtype=torch.uint8), "exp_avg_exps": torch.zeros(3, dtype=torch.uint8),
+                        "exp_avg_sq": torch.zeros(300, dtype=torch.uint8), "exp_avg_sq_exps": torch.zeros(3, dtype=torch.uint8)}},
+          "param_groups": [{**sd["param_groups"][0], "lr": 7.0}]}
+    with pytest.raises(AyoloError, match="GPU"):
+        o.load_state_dict(sd)
+    assert o.param_groups[0]["lr"] == 0.5 and o.param_groups[0]["params"][0] is p
+    assert set(o.state[p]) == set(before) and all(torch.equal(o.state[p][k], v) for k, v in before.items())
+    # what the base class refuses is still the base class's error
+    sd["param_groups"][0]["params"] = [0, 1]
+    with pytest.raises(ValueError, match="parameter group"):
+        o.load_state_dict(sd)
