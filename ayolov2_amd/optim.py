@@ -517,9 +517,24 @@ class AdamW(torch.optim.AdamW):
                     raise _lib.AyoloError(f"{what}: {name}_exps is not one byte per {MOMENT_BLOCK} codes")
 
     def load_state_dict(self, state_dict):
-        self._check_states(state_dict)                     # before anything has changed
-        super().load_state_dict(state_dict)
-        # the base class has cast every state to its parameter's type: take them again as they were saved
+        # Hooks may hand on another state dict, and may change the loaded states: the check sees what all others before the load have
+        # made of it, and the states are in place before the first hook behind it.
+        seen = []
+
+        def check(_, sd):
+            self._check_states(sd)                         # before anything has changed
+            seen.append(sd)
+
+        hooks = (self.register_load_state_dict_pre_hook(check),
+                 self.register_load_state_dict_post_hook(lambda _: self._take_states(seen[-1]), prepend=True))
+        try:
+            super().load_state_dict(state_dict)
+        finally:
+            for h in hooks:
+                h.remove()
+
+    def _take_states(self, state_dict) -> None:
+        """The states as they were saved (the base class has cast every one to its parameter's type)."""
         ids = [i for g in state_dict["param_groups"] for i in g["params"]]
         for i, p in zip(ids, (p for g in self.param_groups for p in g["params"])):
             raw = state_dict["state"].get(i)

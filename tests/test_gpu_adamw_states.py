@@ -129,3 +129,23 @@ def test_refused_loads_change_nothing(bits):
             assert set(o.state[p]) == set(st)
             for k, v in st.items():
                 assert o.state[p][k].dtype == v.dtype and torch.equal(o.state[p][k], v)
+
+
+@pytest.mark.parametrize("bits", [32, 8])
+def test_load_hooks_are_heard(bits):
+    from ayolov2_amd.optim import AdamW
+    a, b = _params("contiguous"), _params("contiguous")
+    oa, ob = AdamW(a, lr=1e-3, state_bits=bits), AdamW(b, lr=1e-3, state_bits=bits)
+    _steps(oa, a, 3, 1)
+    _steps(ob, b, 1, 5)
+    given, seen = oa.state_dict(), []
+    ob.register_load_state_dict_pre_hook(lambda _, sd: given)
+    ob.register_load_state_dict_post_hook(lambda o: seen.extend(o.state[p]["exp_avg"].clone() for p in b))
+    ob.load_state_dict(ob.state_dict())
+    for p, q, s in zip(a, b, seen):
+        for k, v in oa.state[p].items():
+            assert ob.state[q][k].dtype == v.dtype and torch.equal(ob.state[q][k], v)
+        assert torch.equal(s, oa.state[p]["exp_avg"])
+    ob.register_load_state_dict_post_hook(lambda o: [o.state[p]["step"].fill_(40.0) for p in b])
+    ob.load_state_dict(ob.state_dict())
+    assert all(float(ob.state[q]["step"]) == 40.0 for q in b)

@@ -75,3 +75,29 @@ def test_refused_loads_change_nothing():
     sd["param_groups"][0]["params"] = [0, 1]
     with pytest.raises(ValueError, match="parameter group"):
         o.load_state_dict(sd)
+
+
+def test_load_hooks_are_heard():
+    """a hook before the load hands on another state dict; a hook behind it sees the loaded states and changes them for good"""
+    o, p = _adamw()
+    o.step()
+    seen = []
+
+    def other(_, sd):
+        return {"state": {0: {"step": torch.tensor(4.0), "exp_avg": torch.full((300,), 2.0), "exp_avg_sq": torch.full((300,), 3.0)}},
+                "param_groups": sd["param_groups"]}
+
+    def behind(opt):
+        seen.append(float(opt.state[p]["exp_avg"][0]))
+        opt.state[p]["exp_avg"] = torch.full((300,), 5.0)
+
+    o.register_load_state_dict_pre_hook(other)
+    o.register_load_state_dict_post_hook(behind)
+    before = len(o._optimizer_load_state_dict_pre_hooks), len(o._optimizer_load_state_dict_post_hooks)
+    o.load_state_dict(o.state_dict())
+    assert seen == [2.0] and (o.state[p]["exp_avg"] == 5.0).all() and (o.state[p]["exp_avg_sq"] == 3.0).all()
+    # what is handed on is checked too, and nothing stays registered
+    o.register_load_state_dict_pre_hook(lambda _, sd: {"state": {0: {**sd["state"][0], "exp_avg_exps": torch.zeros(3)}}, "param_groups": sd["param_groups"]})
+    with pytest.raises(AyoloError, match="GPU"):
+        o.load_state_dict(o.state_dict())
+    assert (len(o._optimizer_load_state_dict_pre_hooks), len(o._optimizer_load_state_dict_post_hooks)) == (before[0] + 1, before[1])
