@@ -117,6 +117,27 @@ PyObject* rows(PyObject*, PyObject* args) {
     return out;
 }
 
+// unlike(rows, model): the places where both arrays that rows() made hold a tensor and the first one's lies in another shape or
+// memory order than the second one's, which is a dense block
+PyObject* unlike(PyObject*, PyObject* args) {
+    PyObject *a, *b;
+    if (!PyArg_ParseTuple(args, "SS", &a, &b)) return nullptr;
+    const Py_ssize_t n = PyBytes_GET_SIZE(a) / (Py_ssize_t)sizeof(ayolo_tensor);
+    if (PyBytes_GET_SIZE(a) != PyBytes_GET_SIZE(b)) {
+        PyErr_SetString(PyExc_ValueError, "arrays of different lengths");
+        return nullptr;
+    }
+    const auto *x = reinterpret_cast<const ayolo_tensor*>(PyBytes_AS_STRING(a)), *y = reinterpret_cast<const ayolo_tensor*>(PyBytes_AS_STRING(b));
+    PyObject* out = PyList_New(0);
+    for (Py_ssize_t i = 0; out && i < n; ++i) {
+        if (!x[i].present || !y[i].present || y[i].layout == 0 || x[i].layout == y[i].layout) continue;
+        PyObject* k = PyLong_FromSsize_t(i);
+        if (!k || PyList_Append(out, k) != 0) Py_CLEAR(out);
+        Py_XDECREF(k);
+    }
+    return out;
+}
+
 // bump(tensors, given): counts up the version of every tensor of the first list whose entry in the second is not None (kernels
 // write through raw addresses, which autograd's version counters do not see)
 PyObject* bump(PyObject*, PyObject* args) {
@@ -367,6 +388,7 @@ PyObject* bind(PyObject*, PyObject* args) {
 }
 
 PyMethodDef methods[] = {{"rows", rows, METH_VARARGS, "rows(tensors, item=-1) -> bytes of ayolo_tensor"},
+                         {"unlike", unlike, METH_VARARGS, "unlike(rows, model): places in another shape or memory order"},
                          {"bump", bump, METH_VARARGS, "bump(tensors, given): count up the versions of the tensors that are given"},
                          {"layer_norm", layer_norm, METH_VARARGS, "layer_norm(x, weight, bias, eps, residual, dim)"},
                          {"bind", bind, METH_VARARGS, "bind(AyoloError, fwd, bwd, bwd_workspace, last_error)"},

@@ -280,6 +280,11 @@ def _moment_like(p: torch.Tensor, m: torch.Tensor) -> torch.Tensor:
     return torch.empty_like(p, dtype=torch.float32, memory_format=torch.preserve_format).copy_(m)
 
 
+def _in_order_of(p: torch.Tensor, t: torch.Tensor) -> torch.Tensor:
+    """A copy of `t` in parameter `p`'s memory order."""
+    return torch.empty_like(p, dtype=t.dtype, device=t.device, memory_format=torch.preserve_format).copy_(t.detach())
+
+
 def _moment8_like(p: torch.Tensor, m: Moment8, signed: bool) -> Moment8:
     """An 8-bit moment in parameter `p`'s memory order.  The exponents belong to blocks of codes in the codes' OWN order: in another
     one the blocks are others, so the values are taken out and put into codes again."""
@@ -350,14 +355,20 @@ def adamw_step(params: Sequence[torch.Tensor], grads: Sequence[Optional[torch.Te
     if (total_norm is None) != (max_norm is None):
         raise _lib.AyoloError("adamw_step: total_norm and max_norm go together")
     bits8 = isinstance(next((m for m in exp_avgs if m is not None), None), (tuple, list))      # pairs throughout, or tensors
-    rows = _lib.tensor_rows
+    rows, unlike = _lib.tensor_rows, _lib.host().unlike
     L, H = _lib.AdamWList(), _lib.AdamWHyper()
-    L.n, L.p, L.g = n, rows(params, "adamw_step: params"), rows(grads, "adamw_step: grads")
+    P, G = rows(params, "adamw_step: params"), rows(grads, "adamw_step: grads")
+    other = [i for i in unlike(G, P) if grads[i].shape == params[i].shape]
+    if other:                                      # gradients in another memory order than their parameters
+        for i in other:
+            grads[i] = _in_order_of(params[i], grads[i])
+        G = rows(grads, "adamw_step: grads")
+    L.n, L.p, L.g = n, P, G
+    first = 0 if bits8 else -1
+    M, V = rows(exp_avgs, "adamw_step: exp_avgs", first), rows(exp_avg_sqs, "adamw_step: exp_avg_sqs", first)
+    L.m, L.v = M, V
     if bits8:
-        L.m, L.me = rows(exp_avgs, "adamw_step: exp_avgs", 0), rows(exp_avgs, "adamw_step: exp_avgs", 1)
-        L.v, L.ve = rows(exp_avg_sqs, "adamw_step: exp_avg_sqs", 0), rows(exp_avg_sqs, "adamw_step: exp_avg_sqs", 1)
-    else:
-        L.m, L.v = rows(exp_avgs, "adamw_step: exp_avgs"), rows(exp_avg_sqs, "adamw_step: exp_avg_sqs")
+        L.me, L.ve = rows(exp_avgs, "adamw_step: exp_avgs", 1), rows(exp_avg_sqs, "adamw_step: exp_avg_sqs", 1)
     L.step = rows(steps, "adamw_step: steps")
     if torch.is_tensor(lr):
         H.lr_dev = _scalar(lr, dev, "adamw_step", "lr")
@@ -372,19 +383,7 @@ def adamw_step(params: Sequence[torch.Tensor], grads: Sequence[Optional[torch.Te
     H.maximize, H.seed = int(bool(maximize)), int(seed) & 0xFFFFFFFF
     need = int(_lib.lib().ayolo_adamw_workspace(n))
     ws = torch.empty(need, dtype=torch.uint8, device=dev)
-    try:
-        _lib.call_on(dev.index, "ayolo_adamw_step", L, H, ws.data_ptr(), need)
-    except _lib.AyoloError:
-        # a gradient in another memory order than its parameter (the call launches nothing then): laid out like it
-        pi, gi = (np.frombuffer(rows(t, "adamw_step"), dtype=_TENSOR) for t in (params, grads))
-        other = [i for i in np.flatnonzero((gi["present"] != 0) & (pi["layout"] != gi["layout"]) & (pi["layout"] != 0))
-                 if params[i].shape == grads[i].shape]
-        if not other:
-            raise
-        for i in other:
-            grads[i] = SGD._dense_like(params[i], grads[i])
-        L.g = rows(grads, "adamw_step: grads")
-        _lib.call_on(dev.index, "ayolo_adamw_step", L, H, ws.data_ptr(), need)
+    _lib.call_on(dev.index, "ayolo_adamw_step", L, H, ws.data_ptr(), need)
     _lib.host().bump(params, grads)                # written through raw pointers
 
 

@@ -149,3 +149,40 @@ def test_load_hooks_are_heard(bits):
     ob.register_load_state_dict_post_hook(lambda o: [o.state[p]["step"].fill_(40.0) for p in b])
     ob.load_state_dict(ob.state_dict())
     assert all(float(ob.state[q]["step"]) == 40.0 for q in b)
+
+
+def test_gradients_in_another_memory_order():
+    """are laid out like their parameters before the one call that is made; a type that does not fit is refused in any order"""
+    from ayolov2_amd import _lib
+    from ayolov2_amd.optim import adamw_step
+    shape = (16, 8, 3, 3)
+    p0, g0 = _rand(shape, 1), _rand(shape, 2)
+    calls, call_on = [], _lib.call_on
+
+    def counted(device, name, *args):
+        calls.append(name)
+        call_on(device, name, *args)
+
+    res = []
+    _lib.call_on = counted
+    try:
+        for turn in (lambda g: _in_order(g, "channels_last"), lambda g: g, lambda g: g.transpose(0, 3).contiguous().transpose(0, 3)):
+            p, m, v, t = (_in_order(x.cuda(), "channels_last") for x in (p0, torch.zeros(shape), torch.zeros(shape), torch.zeros(())))
+            g = turn(g0.cuda())
+            adamw_step([p, p.clone()], [g, None], [m, None], [v, None], [t, None], lr=1e-2)
+            res.append((p, m, v))
+            with pytest.raises(_lib.AyoloError, match="type is not"):
+                adamw_step([p], [g.half()], [m], [v], [t], lr=1e-2)
+            with pytest.raises(_lib.AyoloError, match="not on a GPU|on device"):
+                adamw_step([p.clone(), p], [_in_order(g, "channels_last"), g.cpu()], [m.clone(), m], [v.clone(), v], [t.clone(), t], lr=1e-2)
+            with pytest.raises(_lib.AyoloError, match="memory order"):
+                adamw_step([p], [g], [m.contiguous()], [v], [t], lr=1e-2)
+    finally:
+        _lib.call_on = call_on
+    for r in res[1:]:
+        assert all(torch.equal(x, y) for x, y in zip(r, res[0]))
+    assert len(calls) == 4 * 3
+    # an expanded gradient
+    p, m, v, t = torch.zeros(5, 7, device="cuda"), torch.zeros(5, 7, device="cuda"), torch.zeros(5, 7, device="cuda"), torch.zeros((), device="cuda")
+    adamw_step([p], [torch.full((), 2.0, device="cuda").expand(5, 7)], [m], [v], [t], lr=0.25, weight_decay=0.0)
+    assert float(t) == 1.0 and ((p + 0.25).abs() <= 0.25 * 16 * ref.U32).all()

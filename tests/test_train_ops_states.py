@@ -101,3 +101,16 @@ def test_load_hooks_are_heard():
     with pytest.raises(AyoloError, match="GPU"):
         o.load_state_dict(o.state_dict())
     assert (len(o._optimizer_load_state_dict_pre_hooks), len(o._optimizer_load_state_dict_post_hooks)) == (before[0] + 1, before[1])
+
+
+def test_places_in_another_memory_order():
+    from ayolov2_amd import _lib
+    host, rows = _lib.host(), lambda ts: _lib.tensor_rows(ts, "x")
+    w = torch.zeros(4, 3, 5, 5)
+    last = w.contiguous(memory_format=torch.channels_last)
+    model = rows([w, last, w, None, w, w[:, :, ::2], torch.zeros(7)])
+    assert host.unlike(rows([w, last, last, w, None, last, torch.zeros(7, dtype=torch.uint8)]), model) == [2]
+    assert host.unlike(rows([w[:, ::2], w[:1].expand(4, 3, 5, 5), w.half(), None, w[:2], w, torch.zeros(8)]), model) == [0, 1, 4, 6]
+    assert host.unlike(b"", b"") == []
+    with pytest.raises(ValueError, match="lengths"):
+        host.unlike(rows([w]), model)
