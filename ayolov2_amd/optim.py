@@ -344,6 +344,14 @@ def adamw_step(params: Sequence[torch.Tensor], grads: Sequence[Optional[torch.Te
     step follows); weight_decay: a number, or a number per tensor.  total_norm with max_norm: gradients are multiplied by
     min(1, max_norm / (total_norm + 1e-6)) on the way.  grad_scale: a device scalar that gradients are divided by; found_inf: a
     device scalar, nothing at all is changed where it is not 0 (torch.amp.GradScaler's pair)."""
+    _adamw(params, grads, exp_avgs, exp_avg_sqs, steps, None, lr, betas, eps, weight_decay, maximize, seed, total_norm, max_norm, grad_scale,
+           found_inf)
+
+
+def _adamw(params, grads, exp_avgs, exp_avg_sqs, steps, relay, lr, betas, eps, weight_decay, maximize, seed, total_norm, max_norm, grad_scale,
+           found_inf) -> None:
+    """adamw_step.  relay(places): puts the moments of these entries into their parameters' memory order, in the lists given here
+    (None: they are refused)."""
     params, grads = list(params), list(grads)
     n = len(params)
     for other, name in ((grads, "grads"), (exp_avgs, "exp_avgs"), (exp_avg_sqs, "exp_avg_sqs"), (steps, "steps")):
@@ -366,6 +374,11 @@ def adamw_step(params: Sequence[torch.Tensor], grads: Sequence[Optional[torch.Te
     L.n, L.p, L.g = n, P, G
     first = 0 if bits8 else -1
     M, V = rows(exp_avgs, "adamw_step: exp_avgs", first), rows(exp_avg_sqs, "adamw_step: exp_avg_sqs", first)
+    if relay is not None:
+        other = [i for i in {*unlike(M, P), *unlike(V, P)} if grads[i] is not None]
+        if other:
+            relay(other)
+            M, V = rows(exp_avgs, "adamw_step: exp_avgs", first), rows(exp_avg_sqs, "adamw_step: exp_avg_sqs", first)
     L.m, L.v = M, V
     if bits8:
         L.me, L.ve = rows(exp_avgs, "adamw_step: exp_avgs", 1), rows(exp_avg_sqs, "adamw_step: exp_avg_sqs", 1)
@@ -440,6 +453,20 @@ class AdamW(torch.optim.AdamW):
             return pairs("exp_avg"), pairs("exp_avg_sq"), [st["step"] for st in sts]
         return [st["exp_avg"] for st in sts], [st["exp_avg_sq"] for st in sts], [st["step"] for st in sts]
 
+    def _relay(self, ps, ms, vs, which) -> None:
+        """Moments into the memory order that their parameters have now (a weight that was made channels-last after its states)."""
+        if torch.cuda.is_current_stream_capturing():
+            raise _lib.AyoloError("ayolov2_amd.optim.AdamW: run one step before capturing: a parameter's memory order has changed")
+        for i in which:
+            p, st = ps[i], self.state[ps[i]]
+            for name, signed, of in (("exp_avg", True, ms), ("exp_avg_sq", False, vs)):
+                if st[name].shape != p.shape:
+                    continue
+                if self.state_bits == 8:
+                    of[i] = st[name], st[name + "_exps"] = _moment8_like(p, Moment8(*of[i]), signed)
+                else:
+                    of[i] = st[name] = _in_order_of(p, st[name])
+
     @torch.no_grad()
     def step(self, closure=None):
         scale, found = getattr(self, "grad_scale", None), getattr(self, "found_inf", None)
@@ -475,9 +502,8 @@ class AdamW(torch.optim.AdamW):
             return loss                                    # no gradients at all
         for r, (key, (ps, grads, ms, vs, ts, lrs, wds)) in enumerate(runs.items()):
             # the seeds of several runs differ, so that their roundings do not repeat one another's
-            adamw_step(ps, grads, ms, vs, ts, lr=lrs[0] if key[3] >= 0 and lrs else lrs, betas=key[0], eps=key[1], weight_decay=wds,
-                       maximize=key[2], seed=self.seed + 0x51F15EED * r, total_norm=norm, max_norm=self.max_norm, grad_scale=scale,
-                       found_inf=found)
+            _adamw(ps, grads, ms, vs, ts, lambda which, a=(ps, ms, vs): self._relay(*a, which), lrs[0] if key[3] >= 0 and lrs else lrs, key[0],
+                   key[1], wds, key[2], self.seed + 0x51F15EED * r, norm, self.max_norm, scale, found)
         return loss
 
     def _check_states(self, state_dict) -> None:

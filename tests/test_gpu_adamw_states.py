@@ -151,6 +151,51 @@ def test_load_hooks_are_heard(bits):
     assert all(float(ob.state[q]["step"]) == 40.0 for q in b)
 
 
+def _turn(ps, order):
+    for p in ps:
+        p.data = _in_order(p.data, order)
+
+
+@pytest.mark.parametrize("bits", [32, 8])
+@pytest.mark.parametrize("src,dst", [("contiguous", "channels_last"), ("channels_last", "contiguous")])
+def test_states_follow_their_parameters_memory_order(src, dst, bits):
+    """Weights that change their memory order between two steps (the executors make weights channels-last at their first forward):
+    as if the states had been saved before and loaded after; with 32-bit moments as if nothing had changed."""
+    from ayolov2_amd.optim import AdamW
+    a, b, c = _params(src), _params(src), _copy_params(_params(src), dst)
+    oa, ob, oc = (AdamW(ps, lr=1e-3, state_bits=bits, seed=3, max_norm=0.5) for ps in (a, b, c))
+    _steps(oa, a, 3, 1)
+    _steps(ob, b, 3, 1)
+    oc.load_state_dict(oa.state_dict())
+    for p, r in zip(a, c):
+        r.data.copy_(p.data)
+    _turn(a, dst)
+    for o, ps in ((oa, a), (ob, b), (oc, c)):
+        _steps(o, ps, 2, 10)
+    for p, q, r in zip(a, b, c):
+        assert torch.equal(p, r) and (bits == 8 or torch.equal(p, q))
+        for k, v in oa.state[p].items():
+            assert torch.equal(v, oc.state[r][k]) and (k not in ("exp_avg", "exp_avg_sq") or v.stride() == p.stride())
+
+
+@pytest.mark.parametrize("bits", [32, 8])
+def test_memory_order_changes_before_a_capture_not_inside(bits):
+    from ayolov2_amd._lib import AyoloError
+    from ayolov2_amd.optim import AdamW
+    ps = _params("contiguous")
+    o = AdamW(ps, lr=1e-3, state_bits=bits)
+    _steps(o, ps, 1, 1)
+    _turn(ps, "channels_last")
+    _grads(ps, 2)
+    torch.cuda.synchronize()
+    with pytest.raises(AyoloError, match="before capturing"):
+        with torch.cuda.graph(torch.cuda.CUDAGraph()):
+            o.step()
+    torch.cuda.synchronize()
+    o.step()
+    assert all(float(o.state[p]["step"]) == 2.0 for p in ps)
+
+
 def test_gradients_in_another_memory_order():
     """are laid out like their parameters before the one call that is made; a type that does not fit is refused in any order"""
     from ayolov2_amd import _lib
