@@ -587,15 +587,20 @@ int check_list(const char* what, const char* name, const ayolo_tensor* t, int n,
     }
     return AYOLO_OK;
 }
-// Whether two of the tensors share memory: sorted by address, does one begin before the last has ended?  A model has some thousand
-// ranges per step in no order; eight bits at a time (and none that all addresses share) sort them in a few us of host time.
+// Whether a tensor that is written shares memory with another one: sorted by address, does a range begin before a written one has
+// ended, or a written one before any has?  Two that are only read may share.  A model has some thousand ranges per step in no order;
+// eight bits at a time (and none that all addresses share) sort them in a few us of host time.
 struct Ranges {
-    struct R { uintptr_t from, to; };
+    struct R { uintptr_t from, to; bool written; };
     std::vector<R> r, other;
-    void add(const ayolo_tensor* t, int n) {
+    void add(const void* p, size_t bytes, bool written) {
+        if (p && bytes) r.push_back(R{(uintptr_t)p, (uintptr_t)p + bytes, written});
+    }
+    static size_t bytes_of(const ayolo_tensor& t) { return (size_t)t.numel * es_of(t.dtype); }
+    void add(const ayolo_tensor* t, int n, bool written) {
         r.reserve(r.size() + n);
         for (int i = 0; i < n; ++i)
-            if (t[i].present && t[i].numel > 0) r.push_back(R{(uintptr_t)t[i].data, (uintptr_t)t[i].data + (uintptr_t)t[i].numel * es_of(t[i].dtype)});
+            if (t[i].present) add(t[i].data, bytes_of(t[i]), written);
     }
     bool overlap() {
         bool ascending = true;
@@ -612,8 +617,12 @@ struct Ranges {
             for (const R& x : r) other[at[x.from >> shift & 255u]++] = x;
             r.swap(other);
         }
-        for (size_t i = 1; i < r.size(); ++i)
-            if (r[i].from < r[i - 1].to) return true;
+        uintptr_t any = 0, written = 0;                    // where the ranges before this one have ended
+        for (const R& x : r) {
+            if (x.from < (x.written ? any : written)) return true;
+            any = std::max(any, x.to);
+            if (x.written) written = std::max(written, x.to);
+        }
         return false;
     }
 };
@@ -711,8 +720,9 @@ extern "C" int ayolo_grad_clip(const ayolo_tensor* grads, int n, const float* no
     if (const int rc = check_list("grad_clip", "grads", grads, n, dev, is_float)) return rc;
     try {
         Ranges r;
-        r.add(grads, n);
-        AY_CHECK_ARG(!r.overlap(), "grad_clip: two of the gradients share memory");
+        r.add(grads, n, true);
+        r.add(norm, sizeof(float), false);
+        AY_CHECK_ARG(!r.overlap(), "grad_clip: two of the gradients, or one and the norm, share memory");
     } catch (...) { ayolo_set_error("grad_clip: out of host memory"); return AYOLO_ENOSPC; }
     hipStream_t s = (hipStream_t)st;
     GJobs P{};
@@ -812,12 +822,14 @@ extern "C" int ayolo_adamw_step(const ayolo_adamw_list* L, const ayolo_adamw_hyp
     }
     try {
         Ranges r;
-        r.add(L->p, n);
-        r.add(L->m, n);
-        r.add(L->v, n);
-        r.add(L->step, n);
-        if (bits8) { r.add(L->me, n); r.add(L->ve, n); }
-        AY_CHECK_ARG(!r.overlap(), "adamw_step: two of the parameters, states or steps share memory");
+        for (const ayolo_tensor* t : {L->p, L->m, L->v, L->step}) r.add(t, n, true);
+        if (bits8) { r.add(L->me, n, true); r.add(L->ve, n, true); }
+        // (a gradient that IS its parameter or moment is read where it is written, by the same thread and before)
+        auto is = [](const ayolo_tensor& a, const ayolo_tensor& b) { return a.data == b.data && Ranges::bytes_of(a) == Ranges::bytes_of(b); };
+        for (int i = 0; i < n; ++i)
+            if (const ayolo_tensor& g = L->g[i]; g.present && !is(g, L->p[i]) && !is(g, L->m[i]) && !is(g, L->v[i])) r.add(&g, 1, false);
+        for (const float* x : {H->lr_dev, H->grad_scale, H->found_inf, H->norm}) r.add(x, sizeof(float), false);
+        AY_CHECK_ARG(!r.overlap(), "adamw_step: two of the parameters, states or steps, or one and what is read, share memory");
     } catch (...) { ayolo_set_error("adamw_step: out of host memory"); return AYOLO_ENOSPC; }
     const size_t need = ayolo_adamw_workspace(n);
     if (!ws || ws_bytes < need) { ayolo_set_error("adamw_step: workspace %zu < %zu", ws_bytes, need); return AYOLO_ENOSPC; }
@@ -887,6 +899,13 @@ extern "C" int ayolo_moment_values(const ayolo_tensor* codes, const ayolo_tensor
         AY_CHECK_ARG(codes[i].present && exps[i].present && out[i].present, "moment_values: tensor %d is missing", i);
         AY_CHECK_ARG(out[i].numel == codes[i].numel && out[i].layout == codes[i].layout && exps[i].numel == cdiv64(codes[i].numel, 128), "moment_values: tensor %d: sizes or memory orders differ", i);
     }
+    try {
+        Ranges r;
+        r.add(codes, n, false);
+        r.add(exps, n, false);
+        r.add(out, n, true);
+        AY_CHECK_ARG(!r.overlap(), "moment_values: two outputs, or one and the moments, share memory");
+    } catch (...) { ayolo_set_error("moment_values: out of host memory"); return AYOLO_ENOSPC; }
     hipStream_t s = (hipStream_t)st;
     UJobs P{};
     return each_launch(P, codes, n,

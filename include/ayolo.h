@@ -234,7 +234,7 @@ typedef struct ayolo_tensor {
 /* Gradient clipping by the 2-norm over all tensors (torch.nn.utils.clip_grad_norm_), beside the optimiser step of
  * scripts/train/yolo_trainer.py:332-338.  ayolo_grad_norm: *norm = sqrt(sum of all squares) / *grad_scale (nullable), summed in
  * fp64 in a fixed order (no atomics), through a workspace of the size that the query gives.  ayolo_grad_clip: every gradient
- * *= min(1, max_norm / (*norm + 1e-6)) in place; refused where two tensors of the list overlap.  n = 0 is allowed. */
+ * *= min(1, max_norm / (*norm + 1e-6)) in place; refused where two tensors of the list overlap, or one and *norm.  n = 0 is allowed. */
 size_t ayolo_grad_norm_workspace(const ayolo_tensor* grads, int n);
 int ayolo_grad_norm(const ayolo_tensor* grads, int n, const float* grad_scale, float* norm, void* ws, size_t ws_bytes,
                     ayolo_stream s);
@@ -246,7 +246,9 @@ int ayolo_grad_clip(const ayolo_tensor* grads, int n, const float* norm, float m
  * stochastically from `seed`, the step count, the tensor's place in the list and the element.  step: one fp32 number per
  * tensor on the device, counted up by the call unless *found_inf != 0.  norm (nullable): gradients are multiplied by
  * min(1, max_norm / (*norm + 1e-6)) on the way, *norm being the norm AFTER division by *grad_scale.  lr_dev (nullable): the
- * learning rate is read from the device (a captured step follows it).  ws: ayolo_adamw_workspace(n) bytes. */
+ * learning rate is read from the device (a captured step follows it).  ws: ayolo_adamw_workspace(n) bytes.  Refused where
+ * something that is written (p, m, v, me, ve, step) shares memory with another tensor or scalar of the call; gradients may share
+ * among themselves, and a gradient may be its own parameter or moment. */
 typedef struct ayolo_adamw_list {
     const ayolo_tensor *p, *g, *m, *v, *me, *ve, *step;
     const float *lr, *weight_decay;       /* host, one per tensor; NULL: the values in ayolo_adamw_hyper */
@@ -261,7 +263,8 @@ typedef struct ayolo_adamw_hyper {
 } ayolo_adamw_hyper;
 size_t ayolo_adamw_workspace(int n);
 int ayolo_adamw_step(const ayolo_adamw_list* list, const ayolo_adamw_hyper* hyper, void* ws, size_t ws_bytes, ayolo_stream s);
-/* The fp32 values that 8-bit moments stand for (is_signed: a first moment, else a second one). */
+/* The fp32 values that 8-bit moments stand for (is_signed: a first moment, else a second one).  Refused where an output shares
+ * memory with another one or with the moments. */
 int ayolo_moment_values(const ayolo_tensor* codes, const ayolo_tensor* exps, const ayolo_tensor* out, int n, int is_signed,
                         ayolo_stream s);
 

@@ -1,0 +1,48 @@
+"""Calls of the training operators on the GPU that their documentation allows or refuses and that a caller makes by the way."""
+import pytest
+import torch
+
+pytestmark = pytest.mark.gpu
+
+
+def _rand(shape, seed, scale=1.0, dt=torch.float32):
+    return (torch.randn(shape, generator=torch.Generator().manual_seed(seed)) * scale).to(dt).cuda()
+
+
+@pytest.mark.parametrize("bits", [32, 8])
+@pytest.mark.parametrize("n", [1, 130, 2048, 5003])
+def test_a_gradient_that_is_its_own_parameter(n, bits):
+    """The gradient of a square's half: the step is the one with a copy of it, bit for bit; also where a moment serves as gradient."""
+    from ayolov2_amd.optim import adamw_step, new_moment8
+
+    def run(own, of):
+        p, t = _rand(n, 1), torch.full((), 3.0, device="cuda")
+        m, v = (new_moment8(p), new_moment8(p)) if bits == 8 else (_rand(n, 2, 0.1), _rand(n, 3, 0.1).square())
+        g = {"p": p, "m": m, "v": v}[of]
+        adamw_step([p], [g if own else g.clone()], [m], [v], [t], lr=1e-2, seed=5)
+        return [p, t, *(m if bits == 8 else [m]), *(v if bits == 8 else [v])]
+
+    for of in ("p",) if bits == 8 else ("p", "m", "v"):
+        for x, y in zip(run(True, of), run(False, of)):
+            assert torch.equal(x, y)
+
+
+def test_what_shares_memory_is_refused():
+    from ayolov2_amd._lib import AyoloError
+    from ayolov2_amd.optim import adamw_step, clip_grads_, new_moment8, unpack_moments
+    big, t = torch.zeros(900, device="cuda"), torch.zeros((), device="cuda")
+    z = lambda: torch.zeros(300, device="cuda")  # noqa: E731
+    with pytest.raises(AyoloError, match="share memory"):
+        adamw_step([big[:300]], [big[1:301]], [z()], [z()], [t], lr=1e-3)
+    with pytest.raises(AyoloError, match="share memory"):
+        adamw_step([z()], [z()], [z()], [z()], [t], lr=t)
+    with pytest.raises(AyoloError, match="share memory"):
+        clip_grads_([big], 1.0, big[5])
+    m = [new_moment8(z()), new_moment8(z())]
+    with pytest.raises(AyoloError, match="share memory"):
+        unpack_moments(m, True, [big[:300], big[200:500]])
+    assert not big.any() and float(t) == 0.0
+    # the same moment twice, the same gradient twice: only read
+    a, b = unpack_moments([m[0], m[0]], True, [big[:300], big[300:600]])
+    adamw_step([big[:300], big[300:600]], [big[600:900], big[600:900]], [z(), z()], [z(), z()], [t, torch.zeros((), device="cuda")], lr=1e-3)
+    assert float(t) == 1.0 and not a.any() and not b.any()
