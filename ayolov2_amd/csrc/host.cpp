@@ -9,9 +9,11 @@
 #include <torch/csrc/autograd/saved_variable.h>
 #include <torch/csrc/Exceptions.h>
 #include <torch/csrc/autograd/python_variable.h>
+#include <torch/csrc/jit/frontend/tracer.h>
 
 #include <ATen/ATen.h>
 #include <c10/core/DeviceGuard.h>
+#include <c10/core/impl/TorchDispatchModeTLS.h>
 #include <c10/hip/HIPStream.h>
 
 #include <stdexcept>
@@ -319,6 +321,18 @@ variable_list norm_with_graph(const Tensor& x, const Tensor& r, const Tensor& w,
     return out;
 }
 
+// Whether torch's calls are recorded to be run later (jit.trace, make_fx and what builds on it): the record would hold the buffers
+// that are made in here and not the kernel that fills them.
+bool recorded() {
+    using c10::impl::TorchDispatchModeKey;
+    using c10::impl::TorchDispatchModeTLS;
+    if (torch::jit::tracer::isTracing()) return true;
+    if (!TorchDispatchModeTLS::any_modes_set()) return false;
+    for (const auto k : {TorchDispatchModeKey::FAKE, TorchDispatchModeKey::PROXY, TorchDispatchModeKey::FUNCTIONAL})
+        if (TorchDispatchModeTLS::get_mode(k).has_value()) return true;
+    return false;
+}
+
 // layer_norm(x, weight, bias, eps, residual, dim): y, or (y, x + residual)
 PyObject* layer_norm(PyObject*, PyObject* args) {
     PyObject *px, *pw, *pb, *pr;
@@ -331,6 +345,7 @@ PyObject* layer_norm(PyObject*, PyObject* args) {
             REFUSE_UNLESS(THPVariable_Check(o), "layer_norm: ", name, " is not a tensor");
             return THPVariable_Unpack(o);
         };
+        REFUSE_UNLESS(!recorded(), "layer_norm: cannot be traced; run the module that holds it eagerly");
         const Tensor x = take(px, "x", true), w = take(pw, "weight", false), b = take(pb, "bias", false), r = take(pr, "residual", false);
         REFUSE_UNLESS(x.is_cuda(), "layer_norm: the HIP path needs a tensor on the GPU (got ", x.device(), "); there is no CPU fallback");
         const int dt = dtype_of(x);

@@ -46,3 +46,38 @@ def test_what_shares_memory_is_refused():
     a, b = unpack_moments([m[0], m[0]], True, [big[:300], big[300:600]])
     adamw_step([big[:300], big[300:600]], [big[600:900], big[600:900]], [z(), z()], [z(), z()], [t, torch.zeros((), device="cuda")], lr=1e-3)
     assert float(t) == 1.0 and not a.any() and not b.any()
+
+
+def test_layer_norm_is_not_traced():
+    """A trace would hold the call's buffers and not its kernel; whoever traces is told so."""
+    from torch.fx.experimental.proxy_tensor import make_fx
+
+    from ayolov2_amd._lib import AyoloError
+    from ayolov2_amd.functional import layer_norm
+    x = _rand((4, 24), 1)
+    with pytest.raises(AyoloError, match="traced"):
+        torch.jit.trace(lambda t: layer_norm(t) + 1.0, x, check_trace=False)
+    for kw in ({}, {"tracing_mode": "fake"}):
+        with pytest.raises(AyoloError, match="traced"):
+            make_fx(lambda t: layer_norm(t) + 1.0, **kw)(x)
+    y = layer_norm(x)                                      # and goes on afterwards
+    assert torch.equal(y, layer_norm(x.clone()))
+
+
+def test_modes_that_only_watch():
+    """a dispatch mode that watches the calls (no tracer) leaves the operator as it is"""
+    from torch.utils._python_dispatch import TorchDispatchMode
+
+    from ayolov2_amd.functional import layer_norm
+
+    class Watch(TorchDispatchMode):
+        def __torch_dispatch__(self, func, types, args=(), kwargs=None):
+            return func(*args, **(kwargs or {}))
+
+    x = _rand((4, 24), 1).requires_grad_()
+    want = layer_norm(x)
+    gw = torch.autograd.grad(want, x, x.detach())[0]
+    with Watch():
+        y = layer_norm(x)
+        g = torch.autograd.grad(y, x, x.detach())[0]
+    assert torch.equal(y, want) and torch.equal(g, gw)

@@ -116,3 +116,11 @@ def test_moment_values_refuses_shared_outputs():
     refused([inside[1199:1499], codes[1]], exps, [big[:300], big[400:700]])
     refused(codes, [exps[0], inside[1600:1603]], [big[:300], big[400:700]])
     refused([codes[0]] * 2, [exps[0]] * 2, [big[:300], big[:300]])
+
+
+def test_layer_norm_is_not_traced():
+    from ayolov2_amd.functional import layer_norm
+    with pytest.raises(_lib.AyoloError, match="traced"):
+        torch.jit.trace(lambda t: layer_norm(t), torch.randn(2, 8), check_trace=False)
+    with pytest.raises(_lib.AyoloError, match="no CPU fallback"):
+        layer_norm(torch.randn(2, 8))
