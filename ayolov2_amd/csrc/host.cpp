@@ -362,6 +362,11 @@ PyObject* layer_norm(PyObject*, PyObject* args) {
         REFUSE_UNLESS(!r.defined() || (r.sizes() == x.sizes() && r.scalar_type() == x.scalar_type() && r.device() == x.device() && r.layout() == at::kStrided),
                       "layer_norm: residual must have x's shape ", x.sizes(), ", type ", x.scalar_type(), " and device ", x.device());
         REFUSE_UNLESS(eps >= 0.0, "layer_norm: eps=", eps);
+        // (a null address would stand for an operand that is not given)
+        for (const auto& p : {std::make_pair(&x, "x"), std::make_pair(&w, "weight"), std::make_pair(&b, "bias"), std::make_pair(&r, "residual")}) {
+            const Tensor& t = *p.first;
+            REFUSE_UNLESS(!t.defined() || t.numel() == 0 || (t.has_storage() && t.storage().data()), "layer_norm: ", p.second, " has no memory of its own");
+        }
         for (const Tensor* t : {&x, &w, &b, &r}) REFUSE_UNLESS(!torch::autograd::isFwGradDefined(*t), "layer_norm has no forward-mode derivative");
         variable_list out;
         auto grad = [](const Tensor& t) { return t.defined() && t.requires_grad(); };

@@ -81,3 +81,31 @@ def test_modes_that_only_watch():
         y = layer_norm(x)
         g = torch.autograd.grad(y, x, x.detach())[0]
     assert torch.equal(y, want) and torch.equal(g, gw)
+
+
+def test_layer_norm_needs_tensors_with_memory():
+    """Transforms' and wrapping tensors have no memory of their own: refused, a gain above all, which would count as none."""
+    from ayolov2_amd._lib import AyoloError
+    from ayolov2_amd.functional import layer_norm
+
+    class Wrapper(torch.Tensor):
+        @staticmethod
+        def __new__(cls, t):
+            return torch.Tensor._make_wrapper_subclass(cls, t.shape, dtype=t.dtype, device=t.device)
+
+        @classmethod
+        def __torch_dispatch__(cls, func, types, args=(), kwargs=None):
+            raise NotImplementedError(str(func))
+
+    x, w = _rand((4, 24), 1), _rand((24,), 2)
+    for kw in (dict(weight=Wrapper(w)), dict(bias=Wrapper(w)), dict(residual=Wrapper(x))):
+        with pytest.raises(AyoloError, match="memory of its own"):
+            layer_norm(x, **kw)
+    with pytest.raises(AyoloError, match="memory of its own"):
+        layer_norm(Wrapper(x), w)
+    with pytest.raises(AyoloError, match="memory of its own"):
+        torch.func.vmap(layer_norm)(_rand((3, 4, 24), 2))
+    with pytest.raises(AyoloError, match="memory of its own"):
+        torch.func.grad(lambda t: layer_norm(t).sum())(x)
+    e = torch.empty(0, 24, device="cuda")                  # nothing to hold is not missing memory
+    assert layer_norm(e, w).shape == (0, 24)
