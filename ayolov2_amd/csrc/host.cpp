@@ -96,7 +96,7 @@ PyObject* rows(PyObject*, PyObject* args) {
             } else {
                 try {
                     const Tensor& t = THPVariable_Unpack(e);
-                    TORCH_CHECK(t.layout() == at::kStrided, "not a strided tensor");
+                    TORCH_CHECK(t.layout() == at::kStrided && !t.is_neg(), "not a strided tensor");
                     row.numel = t.numel();
                     row.dtype = dtype_of(t);
                     row.device = t.is_cuda() ? (int16_t)t.device().index() : (int16_t)-1;
@@ -269,6 +269,8 @@ struct LayerNormBackward : torch::autograd::Node {
             const at::AutoDispatchBelowADInplaceOrView below;
             const c10::DeviceGuard guard(s0.device());
             Tensor x = along(s0, dim);
+            if (dy.is_neg()) dy = dy.resolve_neg();
+            if (q.defined() && q.is_neg()) q = q.resolve_neg();
             dy = along(dy.scalar_type() == x.scalar_type() ? dy : dy.to(x.scalar_type()), dim);
             if (q.defined()) q = along(q.scalar_type() == x.scalar_type() ? q : q.to(x.scalar_type()), dim);
             const int64_t C = x.size(-1), n = x.numel() / C;
@@ -343,7 +345,8 @@ PyObject* layer_norm(PyObject*, PyObject* args) {
         auto take = [](PyObject* o, const char* name, bool needed) -> Tensor {
             if (o == Py_None && !needed) return Tensor();
             REFUSE_UNLESS(THPVariable_Check(o), "layer_norm: ", name, " is not a tensor");
-            return THPVariable_Unpack(o);
+            const Tensor& t = THPVariable_Unpack(o);
+            return t.layout() == at::kStrided && t.is_neg() ? t.resolve_neg() : t;       // (a view with its negation still to be done)
         };
         REFUSE_UNLESS(!recorded(), "layer_norm: cannot be traced; run the module that holds it eagerly");
         const Tensor x = take(px, "x", true), w = take(pw, "weight", false), b = take(pb, "bias", false), r = take(pr, "residual", false);

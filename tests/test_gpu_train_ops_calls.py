@@ -109,3 +109,31 @@ def test_layer_norm_needs_tensors_with_memory():
         torch.func.grad(lambda t: layer_norm(t).sum())(x)
     e = torch.empty(0, 24, device="cuda")                  # nothing to hold is not missing memory
     assert layer_norm(e, w).shape == (0, 24)
+
+
+def test_pending_negation():
+    """A view that stands for its memory's negative (what .imag of a conjugate is): inputs and output gradients of layer norm are
+    what they stand for; the lists' kernels, which read memory, refuse it."""
+    from ayolov2_amd._lib import AyoloError
+    from ayolov2_amd.functional import layer_norm
+    from ayolov2_amd.optim import clip_grads_, grad_norm
+    x, r, gy, w, b = _rand((6, 40), 1), _rand((6, 40), 2), _rand((6, 40), 3), _rand((40,), 4), _rand((40,), 5)
+    neg = torch._neg_view
+    assert neg(x).is_neg()
+
+    def run(x, r, w, b, gy, gs):
+        ops = [t.detach().requires_grad_() for t in (x, r, w, b)]
+        y, s = layer_norm(*[ops[k] for k in (0, 2, 3)], residual=ops[1])
+        return [y, s, *torch.autograd.grad((y, s), ops, (gy, gs))]
+
+    for a, c in zip(run(neg(x), neg(r), neg(w), neg(b), neg(gy), neg(x)), run(-x, -r, -w, -b, -gy, -x)):
+        assert torch.equal(a, c)
+    with torch.no_grad():
+        assert torch.equal(layer_norm(neg(x)), layer_norm(-x))
+    z = torch.complex(x, r).requires_grad_()               # and where autograd itself makes such gradients
+    layer_norm(z.conj().imag).sum().backward()
+    assert torch.isfinite(torch.view_as_real(z.grad)).all()
+    with pytest.raises(AyoloError, match="strided tensor"):
+        grad_norm([neg(x)])
+    with pytest.raises(AyoloError, match="strided tensor"):
+        clip_grads_([neg(x)], 1.0)

@@ -124,3 +124,10 @@ def test_layer_norm_is_not_traced():
         torch.jit.trace(lambda t: layer_norm(t), torch.randn(2, 8), check_trace=False)
     with pytest.raises(_lib.AyoloError, match="no CPU fallback"):
         layer_norm(torch.randn(2, 8))
+
+
+def test_lists_refuse_a_pending_negation():
+    x = torch.randn(6)
+    with pytest.raises(_lib.AyoloError, match="strided tensor"):
+        _lib.tensor_rows([torch._neg_view(x)], "x")
+    assert len(_lib.tensor_rows([-x, torch._neg_view(torch._neg_view(x))], "x")) == 2 * optim._TENSOR.itemsize
