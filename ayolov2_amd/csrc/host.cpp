@@ -140,17 +140,31 @@ PyObject* unlike(PyObject*, PyObject* args) {
     return out;
 }
 
-// bump(tensors, given): counts up the version of every tensor of the first list whose entry in the second is not None (kernels
-// write through raw addresses, which autograd's version counters do not see)
+// bump(tensors, given): counts up the version of every tensor of the first sequence (of every tensor of its pairs) whose entry in the
+// second is not None: kernels write through raw addresses, which autograd's version counters do not see.
 PyObject* bump(PyObject*, PyObject* args) {
-    PyObject *list, *given;
-    if (!PyArg_ParseTuple(args, "O!O!", &PyList_Type, &list, &PyList_Type, &given)) return nullptr;
-    for (Py_ssize_t i = 0; i < PyList_GET_SIZE(list) && i < PyList_GET_SIZE(given); ++i) {
-        PyObject* e = PyList_GET_ITEM(list, i);
-        if (PyList_GET_ITEM(given, i) == Py_None || !THPVariable_Check(e)) continue;
+    PyObject *a, *b;
+    if (!PyArg_ParseTuple(args, "OO", &a, &b)) return nullptr;
+    PyObject* list = PySequence_Fast(a, "a sequence of tensors is needed");
+    PyObject* given = list ? PySequence_Fast(b, "a sequence of tensors is needed") : nullptr;
+    if (!given) {
+        Py_XDECREF(list);
+        return nullptr;
+    }
+    auto one = [](PyObject* e) {
+        if (!THPVariable_Check(e)) return;
         const Tensor& t = THPVariable_Unpack(e);
         if (!t.is_inference()) t.unsafeGetTensorImpl()->bump_version();
+    };
+    for (Py_ssize_t i = 0; i < PySequence_Fast_GET_SIZE(list) && i < PySequence_Fast_GET_SIZE(given); ++i) {
+        if (PySequence_Fast_GET_ITEM(given, i) == Py_None) continue;
+        PyObject* e = PySequence_Fast_GET_ITEM(list, i);
+        if (PyTuple_Check(e)) for (Py_ssize_t k = 0; k < PyTuple_GET_SIZE(e); ++k) one(PyTuple_GET_ITEM(e, k));
+        else if (PyList_Check(e)) for (Py_ssize_t k = 0; k < PyList_GET_SIZE(e); ++k) one(PyList_GET_ITEM(e, k));
+        else one(e);
     }
+    Py_DECREF(list);
+    Py_DECREF(given);
     Py_RETURN_NONE;
 }
 

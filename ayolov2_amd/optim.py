@@ -397,7 +397,8 @@ def _adamw(params, grads, exp_avgs, exp_avg_sqs, steps, relay, lr, betas, eps, w
     need = int(_lib.lib().ayolo_adamw_workspace(n))
     ws = torch.empty(need, dtype=torch.uint8, device=dev)
     _lib.call_on(dev.index, "ayolo_adamw_step", L, H, ws.data_ptr(), need)
-    _lib.host().bump(params, grads)                # written through raw pointers
+    for written in (params, exp_avgs, exp_avg_sqs, steps):        # through raw pointers
+        _lib.host().bump(written, grads)
 
 
 class AdamW(torch.optim.AdamW):

@@ -137,3 +137,23 @@ def test_pending_negation():
         grad_norm([neg(x)])
     with pytest.raises(AyoloError, match="strided tensor"):
         clip_grads_([neg(x)], 1.0)
+
+
+@pytest.mark.parametrize("bits", [32, 8])
+def test_a_step_counts_what_it_writes(bits):
+    """autograd notices that a moment or step count it has saved was changed, as with torch.optim.AdamW"""
+    from ayolov2_amd.optim import adamw_step, new_moment8
+    p = [_rand(300, 1), _rand(300, 2)]
+    make = (lambda: [new_moment8(x) for x in p]) if bits == 8 else (lambda: [torch.zeros_like(x) for x in p])
+    m, v, t = make(), make(), [torch.zeros((), device="cuda") for _ in p]
+    parts = lambda s: list(s) if bits == 8 else [s]  # noqa: E731
+    watched = [[p[k], *parts(m[k]), *parts(v[k]), t[k]] for k in range(2)]
+    before = [[x._version for x in w] for w in watched]
+    adamw_step(p, [_rand(300, 3), None], m, v, tuple(t), lr=1e-2)
+    assert all(x._version > n for x, n in zip(watched[0], before[0])) and [x._version for x in watched[1]] == before[1]
+    if bits == 32:
+        w = torch.ones(300, device="cuda", requires_grad=True)
+        loss = (w * m[0]).sum()
+        adamw_step(p, [_rand(300, 3), None], m, v, t, lr=1e-2)
+        with pytest.raises(RuntimeError, match="modified by an inplace operation"):
+            loss.backward()

@@ -131,3 +131,11 @@ def test_lists_refuse_a_pending_negation():
     with pytest.raises(_lib.AyoloError, match="strided tensor"):
         _lib.tensor_rows([torch._neg_view(x)], "x")
     assert len(_lib.tensor_rows([-x, torch._neg_view(torch._neg_view(x))], "x")) == 2 * optim._TENSOR.itemsize
+
+
+def test_versions_count_up():
+    a, b, c, d = (torch.zeros(3) for _ in range(4))
+    _lib.host().bump([a, (b, c), None, [d, b]], (a, a, a, None))
+    assert [t._version for t in (a, b, c, d)] == [1, 1, 1, 0]
+    with pytest.raises(TypeError):
+        _lib.host().bump(3, [a])
