@@ -229,6 +229,19 @@ def call_on(device: int, name: str, *args) -> None:
 _host = None
 
 
+def _check_host(mod) -> None:
+    """Refuses a helper that was built for another Python or torch than the ones that run (it has no stable ABI)."""
+    import re
+    import sys
+
+    import torch
+    want = "{}.{}".format(*sys.version_info[:2]), re.match(r"\d+\.\d+\.\d+", torch.__version__).group()
+    got = ".".join(mod.built_for_python.split(".")[:2]), mod.built_for_torch
+    if got != want:
+        raise AyoloError("ayolov2_amd/_host.so was built for Python {} and torch {}, running are {} and {}: build it again with "
+                         "`make -C ayolov2_amd/csrc -B PYTHON=...`".format(*got, *want))
+
+
 def host():
     """The compiled helper _host.so (csrc/host.cpp), bound to this library."""
     global _host
@@ -239,6 +252,7 @@ def host():
         except ImportError as e:
             raise AyoloError("ayolov2_amd/_host.so is missing: build it with `python -c 'import __graft_entry__ as g; g.build()'` "
                              f"(or `make -C ayolov2_amd/csrc`). There is no fallback. ({e})")
+        _check_host(mod)
         mod.bind(AyoloError, *(ctypes.cast(f, c_void_p).value for f in (l.ayolo_layer_norm_fwd, l.ayolo_layer_norm_bwd,
                                                                        l.ayolo_layer_norm_bwd_workspace, l.ayolo_last_error)))
         _host = mod

@@ -10,6 +10,7 @@
 #include <torch/csrc/Exceptions.h>
 #include <torch/csrc/autograd/python_variable.h>
 #include <torch/csrc/jit/frontend/tracer.h>
+#include <torch/version.h>
 
 #include <ATen/ATen.h>
 #include <c10/core/DeviceGuard.h>
@@ -434,4 +435,8 @@ PyModuleDef module = {PyModuleDef_HEAD_INIT, "_host", nullptr, -1, methods, null
 
 }  // namespace
 
-PyMODINIT_FUNC PyInit__host() { return PyModule_Create(&module); }
+PyMODINIT_FUNC PyInit__host() {
+    PyObject* m = PyModule_Create(&module);
+    if (m && (PyModule_AddStringConstant(m, "built_for_python", PY_VERSION) != 0 || PyModule_AddStringConstant(m, "built_for_torch", TORCH_VERSION) != 0)) Py_CLEAR(m);
+    return m;
+}
