@@ -108,4 +108,13 @@ typedef _Float16 half2v __attribute__((ext_vector_type(2)));
 typedef float float4v __attribute__((ext_vector_type(4)));
 typedef float float16v __attribute__((ext_vector_type(16)));
 
+// An fp32 result that is then rounded to fp16 stays two roundings: v_fma_mixlo_f16, which rounds once, is chosen for some of the
+// elements of an unrolled loop and not for others, and for one of two routes that are to give the same bits (an activation or
+// gradient that is written by a pass of its own, or formed where it is read).
+template <typename T>
+__device__ __forceinline__ float rounded_f32(float x) {
+    if constexpr (sizeof(T) == 2) asm("" : "+v"(x));
+    return x;
+}
+
 __device__ __forceinline__ float silu_f(float u) { return u / (1.0f + expf(-u)); }

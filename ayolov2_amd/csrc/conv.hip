@@ -1113,7 +1113,7 @@ __global__ __launch_bounds__((GT<T, TM, TPX, NWX>::NT), (NWX == 8 ? 4 : (sizeof(
                 for (int e = 0; e < 8; ++e) {
                     float u = __builtin_fmaf((float)h[e], e < 4 ? a0[e & 3] : a1[e & 3], e < 4 ? b0[e & 3] : b1[e & 3]);
                     if (act) u = u * __builtin_amdgcn_rcpf(1.0f + __builtin_amdgcn_exp2f(u * -1.4426950408889634f));
-                    h[e] = (half_t)u;
+                    h[e] = (half_t)rounded_f32<half_t>(u);
                 }
                 *q = h;
                 if (xst) {
@@ -2371,7 +2371,7 @@ __global__ __launch_bounds__(512, (KC <= 8 ? 4 : 2)) void k_pw(GConvP p) {
                     for (int e = 0; e < 8; ++e) {
                         float u = __builtin_fmaf((float)h[e], e < 4 ? a0_[e & 3] : a1_[e & 3], e < 4 ? b0_[e & 3] : b1_[e & 3]);
                         if (act) u = u * __builtin_amdgcn_rcpf(1.0f + __builtin_amdgcn_exp2f(u * -1.4426950408889634f));
-                        h[e] = (half_t)u;
+                        h[e] = (half_t)rounded_f32<half_t>(u);
                     }
                     *q = h;
                 }
@@ -3305,7 +3305,7 @@ __global__ __launch_bounds__(256, (sizeof(T) == 2 ? 3 : 1)) void k_wgrad(WGradP 
                 for (int e = 0; e < 8; ++e) {
                     float u = __builtin_fmaf((float)h[e], xfa[e], xfb[e]);
                     if (xf_act) u = u * __builtin_amdgcn_rcpf(1.0f + __builtin_amdgcn_exp2f(u * -1.4426950408889634f));
-                    h[e] = (half_t)u;
+                    h[e] = (half_t)rounded_f32<half_t>(u);
                 }
                 *q = h;
             }

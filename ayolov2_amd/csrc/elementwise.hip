@@ -32,13 +32,6 @@ __device__ __forceinline__ void unpack_raw(const uint4& raw, float (&v)[VecT<T>:
 #pragma unroll
     for (int i = 0; i < VecT<T>::VE; ++i) v[i] = (float)e[i];
 }
-// A product and sum whose fp32 result is then rounded to fp16 stays two roundings: v_fma_mixlo_f16, which rounds once, is chosen for
-// some of the pixels of an unrolled loop and not for others, and the transform-on-load kernels' bits would differ from these.
-template <typename T>
-__device__ __forceinline__ float rounded_f32(float x) {
-    if constexpr (sizeof(T) == 2) asm("" : "+v"(x));
-    return x;
-}
 template <typename T>
 __device__ __forceinline__ void store_vec(T* p, const float (&v)[VecT<T>::VE]) {
     uint4 raw;
@@ -773,7 +766,7 @@ __global__ __launch_bounds__(256) void k_bn_bwd_apply2(const T* z, int ldz, T* d
                 uint4 raw;
                 T* e = reinterpret_cast<T*>(&raw);
 #pragma unroll
-                for (int i = 0; i < VE; ++i) e[i] = (T)v[i];
+                for (int i = 0; i < VE; ++i) e[i] = (T)rounded_f32<T>(v[i]);
                 __builtin_amdgcn_raw_buffer_store_b128(__builtin_bit_cast(v4u32_t, raw), rsDz, (unsigned)px * lddzb + cgb, 0, 0);
             } else store_vec<T>(dz + (long long)px * lddz + cg * VE, v);
         };
