@@ -438,10 +438,10 @@ __device__ __forceinline__ void moments(float4v g, const Hyper& h, float4v& m, f
     v = v * h.b2 + g * g * h.c2;
 }
 // Square root and quotient by the hardware's own functions, each 1 ulp: with the two roundings around them below 4 u of the
-// step.  They may take subnormal numbers for zero: a subnormal v (sqrt below 1.1e-19) is nothing beside an ordinary eps, and for
-// a smaller one the exact functions are used.
+// step.  They take subnormal numbers for zero: a root below 2^-63, times c.root, must be nothing beside eps, i.e. at most 2^-26 of
+// it.  So it is from eps = 2.3e-10 on in the first step of b2 = 0.999, 7.3e-12 in the late ones; below, the exact functions are used.
 __device__ __forceinline__ float4v stepped(float4v p, float4v m, float4v v, const Coef& c, float eps) {
-    if (eps >= 1e-12f) {
+    if (eps >= c.root * 0x1p-37f) {
 #pragma unroll
         for (int e = 0; e < 4; ++e) {
             const float d = __builtin_fmaf(__builtin_amdgcn_sqrtf(v[e]), c.root, eps);
