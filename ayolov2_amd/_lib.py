@@ -259,11 +259,11 @@ def host():
     return _host
 
 
-def tensor_rows(tensors, what: str, item: int = -1) -> bytes:
+def tensor_rows(tensors, what: str, item: int = -1, given=None) -> bytes:
     """The ayolo_tensor array of a list of tensors (None: absent).  `item` takes that item of every entry (8-bit moments are
-    (codes, exponents) pairs)."""
+    (codes, exponents) pairs).  `given`: a list; the versions of the tensors whose entry there is not None are counted up."""
     try:
-        return host().rows(tensors, item)
+        return host().rows(tensors, item, given)
     except TypeError as e:
         raise AyoloError(f"{what}: {e}")
 

@@ -583,49 +583,91 @@ int check_list(const char* what, const char* name, const ayolo_tensor* t, int n,
         AY_CHECK_ARG(ok(t[i].dtype), "%s: %s[%d] has an unsupported type", what, name, i);
         AY_CHECK_ARG(t[i].layout != 0, "%s: %s[%d] is not a dense block of memory", what, name, i);
         AY_CHECK_ARG(t[i].numel == 0 || t[i].data, "%s: %s[%d] has no memory", what, name, i);
-        AY_CHECK_ARG((uintptr_t)t[i].data % es_of(t[i].dtype) == 0, "%s: %s[%d] is not aligned to its type", what, name, i);
+        AY_CHECK_ARG(((uintptr_t)t[i].data & (es_of(t[i].dtype) - 1)) == 0, "%s: %s[%d] is not aligned to its type", what, name, i);
     }
     return AYOLO_OK;
 }
 // Whether a tensor that is written shares memory with another one: sorted by address, does a range begin before a written one has
-// ended, or a written one before any has?  Two that are only read may share.  A model has some thousand ranges per step in no order;
-// eight bits at a time (and none that all addresses share) sort them in a few us of host time.
-struct Ranges {
-    struct R { uintptr_t from, to; bool written; };
-    std::vector<R> r, other;
-    void add(const void* p, size_t bytes, bool written) {
-        if (p && bytes) r.push_back(R{(uintptr_t)p, (uintptr_t)p + bytes, written});
+// ended, or a written one before any has?  Two that are only read may share.  A model has some thousand ranges per step.  Lists that
+// are views of a few blocks ascend for long, and where the stretches in which they do lie apart there is nothing to sort; where they
+// do not, ten bits at a time at most, of those in which the addresses differ, sort them in a few us of host time.
+struct Range {
+    uintptr_t from, end;                                   // end: its top bit says that the range is written
+    bool written() const { return end >> 63; }
+    uintptr_t to() const { return end & ~(uintptr_t)0 >> 1; }
+};
+size_t bytes_of(const ayolo_tensor& t) { return (size_t)t.numel * es_of(t.dtype); }
+template <typename F>
+void each_range(const ayolo_tensor* t, int n, bool written, F f) {
+    f(nullptr, 0, false);                                  // (a list of its own: a stretch that went on would span what lies between)
+    for (int i = 0; i < n; ++i)
+        if (t[i].present) f(t[i].data, bytes_of(t[i]), written);
+}
+struct Stretches {
+    static constexpr int MOST = 32;
+    struct { uintptr_t from, to; } of[MOST];
+    int n = 0;
+    uintptr_t from = 0, to = 0;
+    void close() {
+        if (to && n < MOST) of[n].from = from, of[n].to = to;
+        n += to != 0;
     }
-    static size_t bytes_of(const ayolo_tensor& t) { return (size_t)t.numel * es_of(t.dtype); }
-    void add(const ayolo_tensor* t, int n, bool written) {
-        r.reserve(r.size() + n);
-        for (int i = 0; i < n; ++i)
-            if (t[i].present) add(t[i].data, bytes_of(t[i]), written);
+    void add(uintptr_t a, size_t bytes) {                  // nothing (a new list): the stretch ends
+        if (a < to || !to || !bytes) {
+            close();
+            from = a;
+        }
+        to = bytes ? a + bytes : 0;
     }
-    bool overlap() {
-        bool ascending = true;
-        for (size_t i = 1; i < r.size() && ascending; ++i) ascending = r[i].from >= r[i - 1].to;
-        if (ascending) return false;
-        uintptr_t differ = 0;
-        for (const R& x : r) differ |= x.from ^ r[0].from;
-        other.resize(r.size());
-        for (int shift = 0; shift < 64; shift += 8) {
-            if (!(differ >> shift & 255u)) continue;
-            unsigned at[257] = {0};
-            for (const R& x : r) ++at[(x.from >> shift & 255u) + 1];
-            for (int k = 0; k < 256; ++k) at[k + 1] += at[k];
-            for (const R& x : r) other[at[x.from >> shift & 255u]++] = x;
-            r.swap(other);
-        }
-        uintptr_t any = 0, written = 0;                    // where the ranges before this one have ended
-        for (const R& x : r) {
-            if (x.from < (x.written ? any : written)) return true;
-            any = std::max(any, x.to);
-            if (x.written) written = std::max(written, x.to);
-        }
-        return false;
+    bool apart() {
+        close();
+        if (n > MOST) return false;
+        std::sort(of, of + n, [](const auto& x, const auto& y) { return x.from < y.from; });
+        for (int k = 1; k < n; ++k)
+            if (of[k].from < of[k - 1].to) return false;
+        return true;
     }
 };
+void sort_ranges(std::vector<Range>& r) {
+    if (r.size() < 128) {
+        std::sort(r.begin(), r.end(), [](const Range& a, const Range& b) { return a.from < b.from; });
+        return;
+    }
+    uintptr_t differ = 0;
+    for (const Range& x : r) differ |= x.from ^ r[0].from;
+    if (!differ) return;
+    const unsigned low = __builtin_ctzll(differ), width = 64 - __builtin_clzll(differ) - low, passes = (width + 9) / 10;
+    const unsigned bits = (width + passes - 1) / passes, mask = (1u << bits) - 1;
+    std::vector<Range> other(r.size());
+    for (unsigned shift = low, k = 0; k < passes; ++k, shift += bits) {
+        unsigned at[1025];
+        std::fill(at, at + mask + 2, 0u);
+        for (const Range& x : r) ++at[(x.from >> shift & mask) + 1];
+        for (unsigned i = 0; i < mask; ++i) at[i + 1] += at[i];
+        for (const Range& x : r) other[at[x.from >> shift & mask]++] = x;
+        r.swap(other);
+    }
+}
+// each(f): calls f(address, bytes, written) for every range of the call
+template <typename EACH>
+bool overlap(size_t most, EACH each) {
+    Stretches s;
+    each([&](const void* p, size_t bytes, bool) { s.add((uintptr_t)p, p ? bytes : 0); });
+    if (s.apart()) return false;
+    std::vector<Range> r;
+    r.reserve(most);
+    each([&](const void* p, size_t bytes, bool written) {
+        if (p && bytes) r.push_back(Range{(uintptr_t)p, ((uintptr_t)p + bytes) | (uintptr_t)written << 63});
+    });
+    sort_ranges(r);
+    uintptr_t any = 0, written = 0;                        // where the ranges before this one have ended
+    for (const Range& x : r) {
+        if (x.from < (x.written() ? any : written)) return true;
+        any = std::max(any, x.to());
+        if (x.written()) written = std::max(written, x.to());
+    }
+    return false;
+}
 
 // Splits a list into launches.  where(i, off, address): a job's addresses, from element `off` of tensor i on; tag(i, part): its two
 // bits; go(jobs, workgroups) launches what has gathered.
@@ -719,10 +761,12 @@ extern "C" int ayolo_grad_clip(const ayolo_tensor* grads, int n, const float* no
     int dev = -1;
     if (const int rc = check_list("grad_clip", "grads", grads, n, dev, is_float)) return rc;
     try {
-        Ranges r;
-        r.add(grads, n, true);
-        r.add(norm, sizeof(float), false);
-        AY_CHECK_ARG(!r.overlap(), "grad_clip: two of the gradients, or one and the norm, share memory");
+        auto each = [&](auto f) {
+            each_range(grads, n, true, f);
+            f(nullptr, 0, false);
+            f(norm, sizeof(float), false);
+        };
+        AY_CHECK_ARG(!overlap((size_t)n + 1, each), "grad_clip: two of the gradients, or one and the norm, share memory");
     } catch (...) { ayolo_set_error("grad_clip: out of host memory"); return AYOLO_ENOSPC; }
     hipStream_t s = (hipStream_t)st;
     GJobs P{};
@@ -821,15 +865,20 @@ extern "C" int ayolo_adamw_step(const ayolo_adamw_list* L, const ayolo_adamw_hyp
         }
     }
     try {
-        Ranges r;
-        for (const ayolo_tensor* t : {L->p, L->m, L->v, L->step}) r.add(t, n, true);
-        if (bits8) { r.add(L->me, n, true); r.add(L->ve, n, true); }
         // (a gradient that IS its parameter or moment is read where it is written, by the same thread and before)
-        auto is = [](const ayolo_tensor& a, const ayolo_tensor& b) { return a.data == b.data && Ranges::bytes_of(a) == Ranges::bytes_of(b); };
-        for (int i = 0; i < n; ++i)
-            if (const ayolo_tensor& g = L->g[i]; g.present && !is(g, L->p[i]) && !is(g, L->m[i]) && !is(g, L->v[i])) r.add(&g, 1, false);
-        for (const float* x : {H->lr_dev, H->grad_scale, H->found_inf, H->norm}) r.add(x, sizeof(float), false);
-        AY_CHECK_ARG(!r.overlap(), "adamw_step: two of the parameters, states or steps, or one and what is read, share memory");
+        auto is = [](const ayolo_tensor& a, const ayolo_tensor& b) { return a.data == b.data && bytes_of(a) == bytes_of(b); };
+        auto each = [&](auto f) {
+            for (const ayolo_tensor* t : {L->p, L->m, L->v, L->me, L->ve, L->step})
+                if (t) each_range(t, n, true, f);
+            f(nullptr, 0, false);
+            for (int i = 0; i < n; ++i)
+                if (const ayolo_tensor& g = L->g[i]; g.present && !is(g, L->p[i]) && !is(g, L->m[i]) && !is(g, L->v[i])) f(g.data, bytes_of(g), false);
+            for (const float* x : {H->lr_dev, H->grad_scale, H->found_inf, H->norm}) {
+                f(nullptr, 0, false);
+                f(x, sizeof(float), false);
+            }
+        };
+        AY_CHECK_ARG(!overlap((size_t)n * 7 + 4, each), "adamw_step: two of the parameters, states or steps, or one and what is read, share memory");
     } catch (...) { ayolo_set_error("adamw_step: out of host memory"); return AYOLO_ENOSPC; }
     const size_t need = ayolo_adamw_workspace(n);
     if (!ws || ws_bytes < need) { ayolo_set_error("adamw_step: workspace %zu < %zu", ws_bytes, need); return AYOLO_ENOSPC; }
@@ -900,11 +949,12 @@ extern "C" int ayolo_moment_values(const ayolo_tensor* codes, const ayolo_tensor
         AY_CHECK_ARG(out[i].numel == codes[i].numel && out[i].layout == codes[i].layout && exps[i].numel == cdiv64(codes[i].numel, 128), "moment_values: tensor %d: sizes or memory orders differ", i);
     }
     try {
-        Ranges r;
-        r.add(codes, n, false);
-        r.add(exps, n, false);
-        r.add(out, n, true);
-        AY_CHECK_ARG(!r.overlap(), "moment_values: two outputs, or one and the moments, share memory");
+        auto each = [&](auto f) {
+            each_range(codes, n, false, f);
+            each_range(exps, n, false, f);
+            each_range(out, n, true, f);
+        };
+        AY_CHECK_ARG(!overlap((size_t)n * 3, each), "moment_values: two outputs, or one and the moments, share memory");
     } catch (...) { ayolo_set_error("moment_values: out of host memory"); return AYOLO_ENOSPC; }
     hipStream_t s = (hipStream_t)st;
     UJobs P{};

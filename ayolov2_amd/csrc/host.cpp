@@ -43,10 +43,11 @@ std::string text(const A&... a) { return c10::str(a...); }
 uint64_t layout_of(const Tensor& t) {
     if (!t.is_non_overlapping_and_dense()) return 0;
     uint64_t h = 1469598103934665603ull;
-    for (int64_t d = 0; d < t.dim(); ++d) {
-        if (t.size(d) == 1) continue;
-        h = (h ^ (uint64_t)t.size(d)) * 1099511628211ull;
-        h = (h ^ (uint64_t)t.stride(d)) * 1099511628211ull;
+    const at::IntArrayRef size = t.sizes(), stride = t.strides();
+    for (size_t d = 0; d < size.size(); ++d) {
+        if (size[d] == 1) continue;
+        h = (h ^ (uint64_t)size[d]) * 1099511628211ull;
+        h = (h ^ (uint64_t)stride[d]) * 1099511628211ull;
     }
     return h | 1;
 }
@@ -61,13 +62,19 @@ int dtype_of(const Tensor& t) {
     }
 }
 
-// rows(tensors, item=-1) -> bytes: one ayolo_tensor per entry; None gives an absent one; item >= 0 takes that item of each entry
+// rows(tensors, item=-1, given=None) -> bytes: one ayolo_tensor per entry; None gives an absent one; item >= 0 takes that item of each
+// entry.  given, a list: counts up the version of every tensor whose entry there is not None (the kernels write through raw
+// addresses, which autograd's version counters do not see; here, where each tensor is at hand, it costs next to nothing).
 PyObject* rows(PyObject*, PyObject* args) {
-    PyObject* list;
+    PyObject *list, *given = Py_None;
     int item = -1;
-    if (!PyArg_ParseTuple(args, "O|i", &list, &item)) return nullptr;
+    if (!PyArg_ParseTuple(args, "O|iO", &list, &item, &given)) return nullptr;
     if (item > 1) {
         PyErr_SetString(PyExc_ValueError, "item: 0 or 1");
+        return nullptr;
+    }
+    if (given != Py_None && !PyList_Check(given)) {
+        PyErr_SetString(PyExc_TypeError, "given: a list");
         return nullptr;
     }
     PyObject* seq = PySequence_Fast(list, "a sequence of tensors is needed");
@@ -104,6 +111,8 @@ PyObject* rows(PyObject*, PyObject* args) {
                     row.layout = layout_of(t);
                     row.data = row.numel ? t.mutable_data_ptr() : nullptr;
                     row.present = 1;
+                    if (given != Py_None && i < PyList_GET_SIZE(given) && PyList_GET_ITEM(given, i) != Py_None && !t.is_inference())
+                        t.unsafeGetTensorImpl()->bump_version();
                 } catch (const std::exception&) {
                     PyErr_Format(PyExc_TypeError, "entry %zd is not a strided tensor with memory of its own", i);
                     ok = false;
@@ -425,7 +434,7 @@ PyObject* bind(PyObject*, PyObject* args) {
     Py_RETURN_NONE;
 }
 
-PyMethodDef methods[] = {{"rows", rows, METH_VARARGS, "rows(tensors, item=-1) -> bytes of ayolo_tensor"},
+PyMethodDef methods[] = {{"rows", rows, METH_VARARGS, "rows(tensors, item=-1, given=None) -> bytes of ayolo_tensor"},
                          {"unlike", unlike, METH_VARARGS, "unlike(rows, model): places in another shape or memory order"},
                          {"bump", bump, METH_VARARGS, "bump(tensors, given): count up the versions of the tensors that are given"},
                          {"layer_norm", layer_norm, METH_VARARGS, "layer_norm(x, weight, bias, eps, residual, dim)"},

@@ -263,10 +263,9 @@ def unpack_moments(moments: Sequence[Moment8], signed: bool, out: Optional[Seque
         out = [torch.empty_like(m[0], dtype=torch.float32) for m in moments]
     elif len(out) != len(moments):
         raise _lib.AyoloError(f"unpack_moments: {len(out)} outputs for {len(moments)} moments")
-    _lib.call_on(dev.index, "ayolo_moment_values", _lib.tensor_rows(moments, "unpack_moments", 0), _lib.tensor_rows(moments, "unpack_moments", 1),
-                 _lib.tensor_rows(out, "unpack_moments"), len(moments), int(bool(signed)))
     out = list(out)
-    _lib.host().bump(out, out)
+    _lib.call_on(dev.index, "ayolo_moment_values", _lib.tensor_rows(moments, "unpack_moments", 0), _lib.tensor_rows(moments, "unpack_moments", 1),
+                 _lib.tensor_rows(out, "unpack_moments", -1, out), len(moments), int(bool(signed)))
     return out
 
 
@@ -365,7 +364,8 @@ def _adamw(params, grads, exp_avgs, exp_avg_sqs, steps, relay, lr, betas, eps, w
     bits8 = isinstance(next((m for m in exp_avgs if m is not None), None), (tuple, list))      # pairs throughout, or tensors
     rows, unlike = _lib.tensor_rows, _lib.host().unlike
     L, H = _lib.AdamWList(), _lib.AdamWHyper()
-    P, G = rows(params, "adamw_step: params"), rows(grads, "adamw_step: grads")
+    # (what is written through raw pointers counts its versions here, where a gradient is given)
+    P, G = rows(params, "adamw_step: params", -1, grads), rows(grads, "adamw_step: grads")
     other = [i for i in unlike(G, P) if grads[i].shape == params[i].shape]
     if other:                                      # gradients in another memory order than their parameters
         for i in other:
@@ -373,7 +373,7 @@ def _adamw(params, grads, exp_avgs, exp_avg_sqs, steps, relay, lr, betas, eps, w
         G = rows(grads, "adamw_step: grads")
     L.n, L.p, L.g = n, P, G
     first = 0 if bits8 else -1
-    M, V = rows(exp_avgs, "adamw_step: exp_avgs", first), rows(exp_avg_sqs, "adamw_step: exp_avg_sqs", first)
+    M, V = rows(exp_avgs, "adamw_step: exp_avgs", first, grads), rows(exp_avg_sqs, "adamw_step: exp_avg_sqs", first, grads)
     if relay is not None:
         other = [i for i in {*unlike(M, P), *unlike(V, P)} if grads[i] is not None]
         if other:
@@ -381,8 +381,8 @@ def _adamw(params, grads, exp_avgs, exp_avg_sqs, steps, relay, lr, betas, eps, w
             M, V = rows(exp_avgs, "adamw_step: exp_avgs", first), rows(exp_avg_sqs, "adamw_step: exp_avg_sqs", first)
     L.m, L.v = M, V
     if bits8:
-        L.me, L.ve = rows(exp_avgs, "adamw_step: exp_avgs", 1), rows(exp_avg_sqs, "adamw_step: exp_avg_sqs", 1)
-    L.step = rows(steps, "adamw_step: steps")
+        L.me, L.ve = rows(exp_avgs, "adamw_step: exp_avgs", 1, grads), rows(exp_avg_sqs, "adamw_step: exp_avg_sqs", 1, grads)
+    L.step = rows(steps, "adamw_step: steps", -1, grads)
     if torch.is_tensor(lr):
         H.lr_dev = _scalar(lr, dev, "adamw_step", "lr")
     else:
@@ -397,8 +397,6 @@ def _adamw(params, grads, exp_avgs, exp_avg_sqs, steps, relay, lr, betas, eps, w
     need = int(_lib.lib().ayolo_adamw_workspace(n))
     ws = torch.empty(need, dtype=torch.uint8, device=dev)
     _lib.call_on(dev.index, "ayolo_adamw_step", L, H, ws.data_ptr(), need)
-    for written in (params, exp_avgs, exp_avg_sqs, steps):        # through raw pointers
-        _lib.host().bump(written, grads)
 
 
 class AdamW(torch.optim.AdamW):

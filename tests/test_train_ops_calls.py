@@ -139,3 +139,55 @@ def test_versions_count_up():
     assert [t._version for t in (a, b, c, d)] == [1, 1, 1, 0]
     with pytest.raises(TypeError):
         _lib.host().bump(3, [a])
+
+
+@pytest.mark.parametrize("n", [1, 3, 60, 400])
+@pytest.mark.parametrize("shuffled", [False, True])
+def test_overlaps_among_many_ranges(n, shuffled):
+    """Lists in any order, near and far apart (addresses are only compared here): found exactly where a pair of ranges, one of them
+    written, shares a byte."""
+    rng = np.random.default_rng(n + shuffled)
+    lib, ws = _lib.lib(), torch.zeros(8, dtype=torch.uint8)
+    slots = 4 * n                                          # slots of 4 KB, in 16 regions far apart; a tensor fills up to one
+    for trial in range(24):
+        base = np.sort(rng.integers(1 << 20, 1 << 35, 16)).astype(np.uint64) << np.uint64(12)
+        place = rng.permutation(slots) if shuffled else np.arange(slots)
+        addr = (base[place % 16] + (place // 16).astype(np.uint64) * np.uint64(1 << 12) * np.uint64(1 if trial % 2 else 1 << 9)).reshape(4, n)
+        if not shuffled:
+            addr = np.sort(addr, axis=1)
+        lists = []
+        numel = rng.integers(1, 1025, n)
+        for k in range(4):
+            l = np.zeros(n, dtype=optim._TENSOR)
+            l["data"], l["numel"], l["layout"], l["dtype"], l["present"] = addr[k], numel, 77, _lib.F32, 1
+            lists.append(l)
+        step = np.zeros(n, dtype=optim._TENSOR)
+        step["data"], step["numel"], step["layout"], step["dtype"], step["present"] = (1 << 62) + 4 * np.arange(n), 1, 1, _lib.F32, 1
+        if trial % 3 == 0:                                 # one is moved to where another one ends, or a little before
+            k, i, j, m = rng.integers(4), rng.integers(n), rng.integers(n), rng.integers(4)
+            lists[k]["data"][i] = lists[m]["data"][j] + np.uint64(4 * (numel[j] - rng.integers(0, 2)))
+        p, g, m, v = lists
+        spans = [(int(a), int(a) + 4 * int(c), w, (k, i)) for k, (l, w) in enumerate(((p, 1), (g, 0), (m, 1), (v, 1)))
+                 for i, (a, c) in enumerate(zip(l["data"], l["numel"]))]
+        own = {i for i in range(n) if g["data"][i] in (p["data"][i], m["data"][i], v["data"][i])}
+        spans = sorted(s for s in spans if not (s[3][0] == 1 and s[3][1] in own))
+        want, written, any_ = False, 0, 0
+        for a, b, w, _ in spans:
+            want |= a < (any_ if w else written)
+            any_, written = max(any_, b), max(written, b) if w else written
+        L, H = _lib.AdamWList(), _lib.AdamWHyper()
+        L.p, L.g, L.m, L.v, L.step = (l.tobytes() for l in (p, g, m, v, step))
+        L.n, H.beta1, H.beta2, H.eps = n, 0.9, 0.999, 1e-8
+        rc = lib.ayolo_adamw_step(L, H, ws.data_ptr(), 4, None)
+        assert rc == (-1 if want else -3), (trial, lib.ayolo_last_error())
+
+
+def test_rows_count_versions_where_a_gradient_is_given():
+    a, b, c = (torch.zeros(3) for _ in range(3))
+    _lib.tensor_rows([a, b, None], "x", -1, [a, None, a])
+    _lib.tensor_rows([(a, b), (c, b)], "x", 1, [None, a])
+    assert [t._version for t in (a, b, c)] == [1, 1, 0]
+    _lib.tensor_rows([a, b], "x")
+    assert [t._version for t in (a, b, c)] == [1, 1, 0]
+    with pytest.raises(_lib.AyoloError, match="given"):
+        _lib.tensor_rows([a], "x", -1, (a,))
