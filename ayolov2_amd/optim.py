@@ -322,7 +322,7 @@ def _per_tensor(v, n: int, what: str):
     """(number, None), or (0, n floats as bytes) where a number per tensor is given."""
     if isinstance(v, numbers.Real):
         return float(v), None
-    arr = array.array("f", map(float, v))
+    arr = array.array("f", v if type(v) is list else map(float, v))
     if len(arr) != n:
         raise _lib.AyoloError(f"adamw_step: {len(arr)} values of {what} for {n} tensors")
     return 0.0, arr.tobytes()
