@@ -527,11 +527,10 @@ __global__ __launch_bounds__(1024) void k_ln_params(const float* part, int n, in
 }
 
 int cus() {
-    static int n = 0;
-    if (n == 0) {
+    static const int n = [] {                              // (once, whichever thread comes first)
         int dev = 0, v = 0;
-        n = hipGetDevice(&dev) == hipSuccess && hipDeviceGetAttribute(&v, hipDeviceAttributeMultiprocessorCount, dev) == hipSuccess && v > 0 ? v : 256;
-    }
+        return hipGetDevice(&dev) == hipSuccess && hipDeviceGetAttribute(&v, hipDeviceAttributeMultiprocessorCount, dev) == hipSuccess && v > 0 ? v : 256;
+    }();
     return n;
 }
 
