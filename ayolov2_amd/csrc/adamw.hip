@@ -10,7 +10,7 @@
 // ones.  The tensors come as a list on the host and travel BY VALUE in the kernel arguments (up to 4 KB per launch), so nothing is
 // copied to the device, nothing has to be kept between calls, and a captured call replays as it is.  An address is kept as its low
 // half and the number of its 4 GB window, of which a launch knows 16 (an allocator's segments lie far apart), so that a launch
-// takes 330 gradients, 140 tensors with 32-bit and 110 with 8-bit moments: every further launch costs some 4 us of start and drain.
+// takes 332 gradients, 141 tensors with 32-bit and 109 with 8-bit moments: every further launch costs some 4 us of start and drain.
 // A workgroup takes a chunk of one tensor; it finds its tensor by comparing the jobs' first workgroups 64 at a time.
 #include "common.h"
 #include <math.h>
@@ -152,7 +152,7 @@ struct GHead {
     float max_norm;
 };
 typedef Jobs<GHead, 1, CHUNK_GRAD> GJobs;                  // tag: the gradient's type
-static_assert(sizeof(GJobs) <= 4096, "kernel arguments");
+static_assert(sizeof(GJobs) <= 4096 && GJobs::MAX == 332, "kernel arguments");
 
 template <bool FULL, typename T>
 __device__ __forceinline__ double squares(const T* g, unsigned n, unsigned at) {
@@ -252,8 +252,9 @@ __global__ __launch_bounds__(256) void k_grad_clip(GJobs P) {
 // The ranges fit each other: m keeps 2^-17 of its block's largest value, v 2^-33 (sqrt: 2^-16.5), and a v above zero never
 // becomes zero, so that the smallest kept m over the smallest kept sqrt(v) stays a step of ordinary size.
 //
-// Rounding is stochastic, E[stored] = value: at b2 = 0.999 a step moves v by 0.1 % and a 3-bit mantissa by 6 % or nothing, so
-// that rounding to nearest would hold v where it first was.  16 random bits (and a half of the next) per rounding come from a
+// Rounding is stochastic, E[stored] = value (but for a v above zero and below its block's smallest code, which becomes that code):
+// at b2 = 0.999 a step moves v by 0.1 % and a 3-bit mantissa by 6 % or nothing, so that rounding to nearest would hold v where it
+// first was.  16 random bits (and a half of the next) per rounding come from a
 // hash of (seed, t, position of the tensor, element): a call's result depends on its arguments alone.
 constexpr int M_BIAS = 14, V_BIAS = 30, M_LEAST = 1, V_LEAST = 10;      // least E: keeps every value a multiple of 2^-149
 
@@ -404,7 +405,7 @@ struct Hyper {
 };
 // p, g, m, v (and the moments' exponents); tag: which 2^30 elements of its tensor a job is
 template <bool BITS8> using AJobs = Jobs<Hyper, BITS8 ? 6 : 4, CHUNK_ADAMW>;
-static_assert(sizeof(AJobs<false>) <= 4096 && sizeof(AJobs<true>) <= 4096, "kernel arguments");
+static_assert(sizeof(AJobs<false>) <= 4096 && AJobs<false>::MAX == 141 && sizeof(AJobs<true>) <= 4096 && AJobs<true>::MAX == 109, "kernel arguments");
 template <typename T, bool BITS8> struct Tensor;
 template <typename T> struct Tensor<T, false> {
     T* p;

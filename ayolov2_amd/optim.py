@@ -225,8 +225,8 @@ def clip_grads_(grads: Sequence[Optional[torch.Tensor]], max_norm: float, norm: 
 
 
 def clip_grad_norm_(parameters, max_norm: float, norm_type: float = 2.0, error_if_nonfinite: bool = False) -> torch.Tensor:
-    """torch.nn.utils.clip_grad_norm_ for the 2-norm: clips the parameters' ``.grad`` in place (three launches per 330 tensors;
-    gradients that need no clipping are read once and not written) and returns their norm.  Gradients on the CPU go to torch's own function."""
+    """torch.nn.utils.clip_grad_norm_ for the 2-norm: clips the parameters' ``.grad`` in place (two launches per 332 tensors and
+    one for their sum; gradients that need no clipping are read once and not written) and returns their norm.  Gradients on the CPU go to torch's own function."""
     if float(norm_type) != 2.0:
         raise _lib.AyoloError(f"clip_grad_norm_: norm_type={norm_type}: only the 2-norm has a kernel")
     parameters = [parameters] if torch.is_tensor(parameters) else list(parameters)
