@@ -259,7 +259,7 @@ __global__ __launch_bounds__(TS < 128 ? 256 : TS) void k_ln_fwd(Fwd P) {
     }
 }
 
-// Rows longer than the widest team's registers: one workgroup per row, four passes over it (mean, variance, output; the residual
+// Rows longer than the widest team's registers: one workgroup per row, three passes over it (mean, variance, output; the residual
 // sum is formed again in each, from the same roundings).
 template <typename T, int VE, bool RES>
 __global__ __launch_bounds__(1024) void k_ln_fwd_long(Fwd P) {

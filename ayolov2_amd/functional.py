@@ -312,5 +312,5 @@ def layer_norm(x: torch.Tensor, weight: Optional[torch.Tensor] = None, bias: Opt
     ``(y, s)`` is returned: the sum and the norm of a pre-norm block in one pass, each with its gradient.  weight / bias: (C,),
     floating, each optional.  Rows may have any strides and any alignment as long as `dim` is contiguous in memory; otherwise x
     is copied first.  Differentiable once, in x, residual, weight and bias; gradients have the inputs' types and the same bits
-    in every run."""
+    in every run.  Not traceable (jit.trace, make_fx), nor under torch.func's transforms: refused."""
     return _lib.host().layer_norm(x, weight, bias, float(eps), residual, dim)

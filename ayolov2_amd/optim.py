@@ -226,7 +226,8 @@ def clip_grads_(grads: Sequence[Optional[torch.Tensor]], max_norm: float, norm: 
 
 def clip_grad_norm_(parameters, max_norm: float, norm_type: float = 2.0, error_if_nonfinite: bool = False) -> torch.Tensor:
     """torch.nn.utils.clip_grad_norm_ for the 2-norm: clips the parameters' ``.grad`` in place (two launches per 332 tensors and
-    one for their sum; gradients that need no clipping are read once and not written) and returns their norm.  Gradients on the CPU go to torch's own function."""
+    one for their sum; gradients that need no clipping are read once and not written) and returns their norm.  Gradients on the CPU go to
+    torch's own function."""
     if float(norm_type) != 2.0:
         raise _lib.AyoloError(f"clip_grad_norm_: norm_type={norm_type}: only the 2-norm has a kernel")
     parameters = [parameters] if torch.is_tensor(parameters) else list(parameters)
@@ -242,7 +243,8 @@ def clip_grad_norm_(parameters, max_norm: float, norm_type: float = 2.0, error_i
 
 # --------------------------------------------------------------------------------------------------------------- AdamW
 class Moment8(NamedTuple):
-    """A moment in 8 bits: one code per element in the parameter's shape and memory order, one exponent per MOMENT_BLOCK codes."""
+    """A moment in 8 bits: one code per element in the parameter's shape and memory order, one exponent per MOMENT_BLOCK codes in that
+    order (codes that are copied into another one no longer fit their exponents)."""
     codes: torch.Tensor
     exps: torch.Tensor
 
@@ -336,7 +338,8 @@ def adamw_step(params: Sequence[torch.Tensor], grads: Sequence[Optional[torch.Te
     """One AdamW step (torch.optim.AdamW's arithmetic) over lists of tensors, in place, in a few launches for all of them.
 
     params / grads: fp32, fp16 or bf16 on one GPU, a gradient of its parameter's type (None: that entry stays as it is); dense
-    blocks of memory, states in the parameter's memory order.  16-bit parameters are rounded to nearest: what is below half a
+    blocks of memory, states in the parameter's memory order (gradients are laid out like it where they are not); what is written
+    shares memory with nothing else of the call.  16-bit parameters are rounded to nearest: what is below half a
     step of theirs is lost, so keep fp32 masters for long training.  exp_avgs / exp_avg_sqs: fp32 tensors, or Moment8 pairs
     (new_moment8), rounded stochastically from `seed`, the step, the entry's place in the list and the element.  steps: one fp32
     number per entry on the device, counted up here.  lr: a number, a number per tensor, or a device scalar (which a captured
@@ -407,7 +410,8 @@ class AdamW(torch.optim.AdamW):
     ``max_norm`` clips the gradients' global 2-norm inside the step, without writing them.  ``step`` counts on the device, so
     GradScaler's skipped steps do not count and need no host sync, and a step can be captured (after one eager step, which makes
     the states; a learning rate that changes between replays is given as a device scalar).  32-bit state dicts and
-    torch.optim.AdamW's load into each other; an 8-bit state dict also loads into a 32-bit optimiser.  CPU parameters fall back
+    torch.optim.AdamW's load into each other; an 8-bit state dict also loads into a 32-bit optimiser.  States are brought into their
+    parameter's memory order when they are loaded and when it changes (8-bit ones are rounded to nearest once).  CPU parameters fall back
     to torch's own arithmetic (32-bit states)."""
     _step_supports_amp_scaling = True
 
