@@ -599,10 +599,10 @@ struct Range {
 };
 size_t bytes_of(const ayolo_tensor& t) { return (size_t)t.numel * es_of(t.dtype); }
 template <typename F>
-void each_range(const ayolo_tensor* t, int n, bool written, F f) {
+void each_range(const ayolo_tensor* t, int n, bool written, F f, const ayolo_tensor* given = nullptr) {
     f(nullptr, 0, false);                                  // (a list of its own: a stretch that went on would span what lies between)
     for (int i = 0; i < n; ++i)
-        if (t[i].present) f(t[i].data, bytes_of(t[i]), written);
+        if (t[i].present && (!given || given[i].present)) f(t[i].data, bytes_of(t[i]), written);
 }
 struct Stretches {
     static constexpr int MOST = 32;
@@ -870,7 +870,7 @@ extern "C" int ayolo_adamw_step(const ayolo_adamw_list* L, const ayolo_adamw_hyp
         auto is = [](const ayolo_tensor& a, const ayolo_tensor& b) { return a.data == b.data && bytes_of(a) == bytes_of(b); };
         auto each = [&](auto f) {
             for (const ayolo_tensor* t : {L->p, L->m, L->v, L->me, L->ve, L->step})
-                if (t) each_range(t, n, true, f);
+                if (t) each_range(t, n, true, f, L->g);    // (without a gradient, nothing is written)
             f(nullptr, 0, false);
             for (int i = 0; i < n; ++i)
                 if (const ayolo_tensor& g = L->g[i]; g.present && !is(g, L->p[i]) && !is(g, L->m[i]) && !is(g, L->v[i])) f(g.data, bytes_of(g), false);

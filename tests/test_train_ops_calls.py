@@ -191,3 +191,17 @@ def test_rows_count_versions_where_a_gradient_is_given():
     assert [t._version for t in (a, b, c)] == [1, 1, 0]
     with pytest.raises(_lib.AyoloError, match="given"):
         _lib.tensor_rows([a], "x", -1, (a,))
+
+
+def test_entries_without_a_gradient_share_what_they_like():
+    """nothing of theirs is written"""
+    l = _lists(3)
+    l["g"][1] = l["g"][2] = None
+    l["p"][2] = l["p"][1]
+    l["step"][2] = l["step"][1]
+    l["m"][1] = l["g"][0]
+    _free(_adamw(**l))
+    l["p"][2] = l["p"][0]
+    _free(_adamw(**l))
+    l["g"][2] = torch.zeros(300)
+    _shares(_adamw(**l))
