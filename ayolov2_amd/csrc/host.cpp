@@ -261,6 +261,18 @@ Norm norm_forward(const Tensor& x0, const Tensor& r0, const Tensor& w0, const Te
     return o;
 }
 
+// Whether torch's calls are recorded to be run later (jit.trace, make_fx and what builds on it): the record would hold the buffers
+// that are made in here and not the kernel that fills them.
+bool recorded() {
+    using c10::impl::TorchDispatchModeKey;
+    using c10::impl::TorchDispatchModeTLS;
+    if (torch::jit::tracer::isTracing()) return true;
+    if (!TorchDispatchModeTLS::any_modes_set()) return false;
+    for (const auto k : {TorchDispatchModeKey::FAKE, TorchDispatchModeKey::PROXY, TorchDispatchModeKey::FUNCTIONAL})
+        if (TorchDispatchModeTLS::get_mode(k).has_value()) return true;
+    return false;
+}
+
 // Its edges: x, residual, weight, bias.
 struct LayerNormBackward : torch::autograd::Node {
     torch::autograd::SavedVariable s, w, mean, rstd;
@@ -279,6 +291,7 @@ struct LayerNormBackward : torch::autograd::Node {
 
     variable_list apply(variable_list&& grads) override {
         const std::lock_guard<std::mutex> lock(mutex_);
+        REFUSE_UNLESS(!recorded(), "layer_norm: its backward cannot be traced");
         const bool nx = task_should_compute_output(0), nr = task_should_compute_output(1), nw = task_should_compute_output(2),
                    nb = task_should_compute_output(3);
         Tensor dy = grads[0], q = grads.size() > 1 ? grads[1] : Tensor(), dx, dw, db;
@@ -345,18 +358,6 @@ variable_list norm_with_graph(const Tensor& x, const Tensor& r, const Tensor& w,
     node->mean = torch::autograd::SavedVariable(o.mean, false);
     node->rstd = torch::autograd::SavedVariable(o.rstd, false);
     return out;
-}
-
-// Whether torch's calls are recorded to be run later (jit.trace, make_fx and what builds on it): the record would hold the buffers
-// that are made in here and not the kernel that fills them.
-bool recorded() {
-    using c10::impl::TorchDispatchModeKey;
-    using c10::impl::TorchDispatchModeTLS;
-    if (torch::jit::tracer::isTracing()) return true;
-    if (!TorchDispatchModeTLS::any_modes_set()) return false;
-    for (const auto k : {TorchDispatchModeKey::FAKE, TorchDispatchModeKey::PROXY, TorchDispatchModeKey::FUNCTIONAL})
-        if (TorchDispatchModeTLS::get_mode(k).has_value()) return true;
-    return false;
 }
 
 // layer_norm(x, weight, bias, eps, residual, dim): y, or (y, x + residual)

@@ -157,3 +157,15 @@ def test_a_step_counts_what_it_writes(bits):
         adamw_step(p, [_rand(300, 3), None], m, v, t, lr=1e-2)
         with pytest.raises(RuntimeError, match="modified by an inplace operation"):
             loss.backward()
+
+
+def test_layer_norms_backward_is_not_traced():
+    """a gradient taken inside a trace, of a norm computed before it"""
+    from torch.fx.experimental.proxy_tensor import make_fx
+
+    from ayolov2_amd.functional import layer_norm
+    x = _rand((4, 24), 1).requires_grad_()
+    y = layer_norm(x)
+    with pytest.raises(RuntimeError, match="traced"):
+        make_fx(lambda g: torch.autograd.grad(y, x, g, retain_graph=True)[0] + 1.0)(_rand((4, 24), 2))
+    assert torch.isfinite(torch.autograd.grad(y, x, x.detach())[0]).all()
