@@ -236,7 +236,7 @@ def _check_host(mod) -> None:
 
     import torch
     want = "{}.{}".format(*sys.version_info[:2]), re.match(r"\d+\.\d+\.\d+", torch.__version__).group()
-    got = ".".join(mod.built_for_python.split(".")[:2]), mod.built_for_torch
+    got = ".".join(getattr(mod, "built_for_python", "?").split(".")[:2]), getattr(mod, "built_for_torch", "?")
     if got != want:
         raise AyoloError("ayolov2_amd/_host.so was built for Python {} and torch {}, running are {} and {}: build it again with "
                          "`make -C ayolov2_amd/csrc -B PYTHON=...`".format(*got, *want))

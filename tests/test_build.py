@@ -44,4 +44,6 @@ def test_a_helper_of_another_build_is_refused():
     for py, tv in (("3.99.1", mod.built_for_torch), (mod.built_for_python, "1.0.0")):
         with pytest.raises(_lib.AyoloError, match="build it again"):
             _lib._check_host(types.SimpleNamespace(built_for_python=py, built_for_torch=tv))
+    with pytest.raises(_lib.AyoloError, match="build it again"):
+        _lib._check_host(types.SimpleNamespace())          # built before it said for what
     _lib._check_host(mod)
