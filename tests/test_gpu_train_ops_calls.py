@@ -169,3 +169,83 @@ def test_layer_norms_backward_is_not_traced():
     with pytest.raises(RuntimeError, match="traced"):
         make_fx(lambda g: torch.autograd.grad(y, x, g, retain_graph=True)[0] + 1.0)(_rand((4, 24), 2))
     assert torch.isfinite(torch.autograd.grad(y, x, x.detach())[0]).all()
+
+
+@pytest.mark.parametrize("leaf", [True, False])
+def test_the_residual_is_the_input_itself(leaf):
+    """and gradients that the norm hands to two leaves are two tensors"""
+    from ayolov2_amd.functional import layer_norm
+    base, gy, gs = _rand((7, 96), 1), _rand((7, 96), 2), _rand((7, 96), 3)
+    a = base.clone().requires_grad_()
+    x = a if leaf else a * 1.0
+    y, s = layer_norm(x, residual=x)
+    assert torch.equal(s, base + base)
+    torch.autograd.backward((y, s), (gy, gs))
+    b = (base + base).requires_grad_()
+    ds = torch.autograd.grad(layer_norm(b), b, gy)[0] + gs
+    # 2 ds, ds rounded once more here than there: 2 u of its terms
+    assert ((a.grad.double() - 2 * ds.double()).abs() <= 4 * 2.0 ** -24 * (2 * ds.abs() + 2 * gs.abs()).double()).all()
+    p, q = base.clone().requires_grad_(), gs.clone().requires_grad_()
+    y, s = layer_norm(p, residual=q)
+    torch.autograd.backward((y, s), (gy, gs))
+    assert torch.equal(p.grad, q.grad) and p.grad.data_ptr() != q.grad.data_ptr()
+    kept = gs.clone()
+    p, q = base.clone().requires_grad_(), base.clone().requires_grad_()
+    layer_norm(p, residual=q)[1].backward(gs)              # only the sum: its gradient goes on as it is
+    p.grad.zero_()
+    assert torch.equal(q.grad, kept) and torch.equal(gs, kept)
+
+
+def test_a_model_with_a_layer_norm_row_in_use():
+    """evaluation, evaluation with augmentations, a 16-bit copy, the moving average and a clipped step, against the same model with
+    the norm in torch operations"""
+    import copy
+    import os
+
+    import yaml
+
+    import ayolov2_amd
+    from ayolov2_amd import LayerNorm, YOLOModel
+    from ayolov2_amd.losses import ComputeLoss
+    from ayolov2_amd.optim import AdamW
+    from ayolov2_amd.trainer import ModelEMA, training_step
+    from ayolov2_amd.tta import inference_with_tta
+    cfg = yaml.safe_load(open(os.path.join(os.path.dirname(ayolov2_amd.__file__), "configs", "yolov5n.yaml")))
+    cfg["backbone"].append([-1, 1, "LayerNorm", []])
+    at = len(cfg["backbone"]) - 1
+    cfg["head"][-1][0] = [at if f == at - 1 else f for f in cfg["head"][-1][0]]
+    hyp = dict(box=0.05, cls=0.5, cls_pw=1.0, obj=1.0, obj_pw=1.0, anchor_t=4.0, fl_gamma=0.0, label_smoothing=0.0)
+    torch.manual_seed(0)
+    m = YOLOModel(cfg).cuda()
+    m.hyp, m.gr = hyp, 1.0
+
+    def torchs(model):
+        other = copy.deepcopy(model)
+        for n in other.modules():
+            if isinstance(n, LayerNorm):
+                n.forward = lambda t, n=n: torch.nn.functional.layer_norm(
+                    t.permute(0, 2, 3, 1).float(), (n.weight.shape[0],), n.weight.float(), n.bias.float(), n.eps).permute(0, 3, 1, 2).to(t.dtype)
+        return other
+
+    x = torch.rand(2, 3, 64, 96, generator=torch.Generator().manual_seed(1)).cuda()
+    m.eval()
+    with torch.no_grad():
+        for a, c in ((m(x)[0], torchs(m)(x)[0]), (inference_with_tta(m, x, (1.0, 0.83), (None, 3))[0], inference_with_tta(torchs(m), x, (1.0, 0.83), (None, 3))[0])):
+            # as the fp32 model tests: 1e-4 of the largest value
+            assert a.shape == c.shape and float((a - c).abs().max()) <= 1e-4 * float(c.abs().max())
+        h = copy.deepcopy(m).half()
+        a, c = h(x.half())[0].float(), torchs(h)(x.half())[0].float()
+        # fp16 activations from the norm on: some 10 layers of half a step (2^-11) each
+        assert torch.isfinite(a).all() and float((a - c).abs().max()) <= 10 * 2.0 ** -11 * float(c.abs().max())
+    m.train()
+    ema = ModelEMA(m)
+    before = {k: v.clone() for k, v in m.state_dict().items()}
+    o = AdamW(m.parameters(), lr=1e-3, state_bits=8)
+    targets = torch.tensor([[0, 3, 0.5, 0.5, 0.4, 0.3], [1, 7, 0.3, 0.6, 0.2, 0.5]]).cuda()
+    training_step(m, ComputeLoss(m), o, torch.amp.GradScaler("cuda", init_scale=64.0), x, targets, max_norm=0.5, ema=ema)
+    name = next(k for k in before if k.startswith(f"model.{at}.") and k.endswith("weight"))
+    after = m.state_dict()[name]
+    assert not torch.equal(after, before[name]) and torch.isfinite(after).all()
+    d = ema.decay(1)
+    # one step of the average: two products and a sum
+    assert torch.allclose(ema.ema.state_dict()[name], d * before[name] + (1 - d) * after, rtol=4 * 2.0 ** -24, atol=4 * 2.0 ** -24)
